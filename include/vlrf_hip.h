@@ -43,6 +43,9 @@ extern "C" {
 #define VLRF_HIP_KV_F32   0
 #define VLRF_HIP_KV_F16   1   /* the reference's f32_to_f16 (kv_cache.hpp:68-97), bit-exact */
 #define VLRF_HIP_KV_Q8_0  2
+/* This library's own, no KVCacheDType of the reference: Q4_0 blocks (as VLRF_HIP_DT_Q4_0)
+ * of 32 consecutive elements of a head's row, 4.5 bits an element. */
+#define VLRF_HIP_KV_Q4_0  3
 
 typedef struct vlrf_hip_ctx*    vlrf_hip_ctx_t;
 typedef struct vlrf_hip_weight* vlrf_hip_weight_t;
@@ -90,11 +93,12 @@ int vlrf_hip_attn_f32(vlrf_hip_ctx_t ctx, const float* Q, const float* K, const 
                       float* O, int n_h, int T, int ctx_len, int d_h, float scale, int causal);
 
 /* ============================================================================
- * KV cache (reference kv_cache.hpp:14-17,132-293), dtype VLRF_HIP_KV_F32, _F16 or
- * _Q8_0 (per token row).  Device layout: per layer, K and V elements
- * [n_kv_heads][max_seq][d_head] (head-major, so one head's history is one
- * contiguous stream): f32, f16 bits, or int8 codes with one f32 scale per
- * token row for K and for V.
+ * KV cache (reference kv_cache.hpp:14-17,132-293), dtype VLRF_HIP_KV_F32, _F16,
+ * _Q8_0 (per token row) or _Q4_0 (d_head a multiple of 32).  Device layout: per
+ * layer, K and V elements [n_kv_heads][max_seq][d_head] (head-major, so one head's
+ * history is one contiguous stream): f32, f16 bits, or int8 codes with one f32 scale
+ * per token row for K and for V; Q4_0 head-major too, codes and f16 scales in the
+ * order its kernels load them in (csrc/kernels/kv4_layout.hpp).
  * ========================================================================== */
 /* Replaces: KVCache::KVCache (kv_cache.hpp:152-177), per layer. */
 int vlrf_hip_kv_create(vlrf_hip_ctx_t ctx, int n_layers, int max_seq, int n_kv_heads,
@@ -107,13 +111,19 @@ int vlrf_hip_kv_used(vlrf_hip_kv_t kv, int layer);
 /* Replaces: KVCache::append (kv_cache.hpp:215-251): stores T rows of device
  * f32 k/v [T, n_kv_heads*d_head] at positions [used, used+T), then used += T,
  * bit-exactly as the reference: Q8_0 quantize_row_q8_0 (kv_cache.hpp:102-117),
- * F16 its f32_to_f16 (:68-97, half-up rounding, flush to zero), F32 a copy.
+ * F16 its f32_to_f16 (:68-97, half-up rounding, flush to zero), F32 a copy; Q4_0
+ * each block as vlrf_quantize_q4_0, except that a block with an infinity or a NaN
+ * gets a NaN scale: it reads back as NaN, and so does what attends to it.
  * VLRF_HIP_ERR_OVERFLOW when used+T > max_seq (the reference throws). */
 int vlrf_hip_kv_append(vlrf_hip_kv_t kv, int layer, const float* k, const float* v, int T);
+/* Forgets the rows of `layer` from n on, 0 <= n <= used (drafted tokens that were
+ * refused, a prompt that goes on differently): used = n, appends go on there. */
+int vlrf_hip_kv_truncate(vlrf_hip_kv_t kv, int layer, int n);
 /* Copies rows [row0,row0+n) of `layer` to host in the reference's token-major
  * layout: k_q/v_q [n, n_kv_heads*d_head] elements of the cache's dtype (int8
  * codes, f16 bits or f32; the pointers address bytes), k_s/v_s f32 [n] row
- * scales for Q8_0 (ignored otherwise; any pointer may be NULL). Synchronous. */
+ * scales for Q8_0 (ignored otherwise; any pointer may be NULL).  Q4_0: rows of
+ * n_kv_heads*d_head/32 GGUF blocks of 18 bytes. Synchronous. */
 int vlrf_hip_kv_read(vlrf_hip_kv_t kv, int layer, int row0, int n, int8_t* k_q, int8_t* v_q,
                      float* k_s, float* v_s);
 /* Replaces: KVCache::dequant_into (kv_cache.hpp:259-286): device f32
@@ -139,6 +149,15 @@ int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out
  * (allocated at vlrf_hip_init).  Calls that overlap on one GPU race. */
 int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, float* out,
                                  int n_heads, int ctx_len, float scale);
+/* Causal attention of T query rows, the last T of ctx_len tokens, over a Q4_0 cache
+ * (a prompt in chunks, or drafted tokens checked together; their K/V are appended
+ * first): q and out device f32 [T, n_heads*d_head], q already rotated; row t sees the
+ * keys [0, ctx_len - T + t].  1 <= T <= ctx_len <= max_seq; d_head 64 or 128; any
+ * n_heads / n_kv_heads.  Other cache dtypes are VLRF_HIP_ERR_ARG.  f32-class: q and
+ * the weights enter the matrix cores in two f16 pieces (22 bits) beside the cache's
+ * exact codes, sums and softmax in f32.  attn_decode over a Q4_0 cache is T = 1. */
+int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T,
+                        int ctx_len, float scale);
 
 /* ============================================================================
  * Quantized linear: y[M,N] = x[M,K] . W[N,K]^T with W in a GGUF block format.

@@ -1,0 +1,65 @@
+"""The 4-bit KV cache's layout (csrc/kernels/kv4_layout.hpp) on the CPU: every
+code byte and scale of every row has a place of its own inside the head's
+arrays, and the entry points refuse what they can see without a device."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+
+import vlrf_amd as V
+from vlrf_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+SOURCE = r"""
+#include "vlrf_amd/csrc/kernels/kv4_layout.hpp"
+#include <cstdio>
+#include <set>
+using namespace vlrf_hip;
+int main() {
+    for (int d : {32, 64, 96, 128, 256})
+        for (int seq : {1, 31, 32, 33, 200}) {
+            std::set<size_t> k, v, s;
+            for (int t = 0; t < seq; ++t) {
+                if (kv4::key_of(kv4::lane_group(t), kv4::slot(t)) != t % 32) return 1;
+                for (int b = 0; b < d / 32; ++b) {
+                    s.insert(kv4::scale(t, b, d));
+                    for (int i = 0; i < 16; ++i) {
+                        k.insert(kv4::k_word(t, i / 4, b, d) + i % 4);
+                        v.insert(kv4::v_byte(t, i, b, d));
+                    }
+                }
+            }
+            const size_t n = (size_t)seq * d / 2, m = (size_t)seq * d / 32;
+            if (k.size() != n || v.size() != n || s.size() != m) return 2;
+            if (*k.rbegin() >= kv4::head_codes(seq, d) || *v.rbegin() >= kv4::head_codes(seq, d)) return 3;
+            if (*s.rbegin() >= kv4::head_scales(seq, d)) return 4;
+        }
+    // Past 32 bits: 100 million rows of 128.
+    const int t = 99999999;
+    if (kv4::k_word(t, 3, 3, 128) != (size_t)t * 64 + 60 || kv4::k_word(t, 3, 3, 128) >= kv4::head_codes(t + 1, 128)) return 5;
+    if (kv4::v_byte(t, 15, 3, 128) >= kv4::head_codes(t + 1, 128) || kv4::v_byte(t, 15, 3, 128) < ((size_t)5 << 30)) return 6;
+    if (kv4::scale(t, 3, 128) >= kv4::head_scales(t + 1, 128)) return 7;
+    return 0;
+}
+"""
+
+
+def test_every_code_and_scale_has_its_own_place(tmp_path):
+    if not shutil.which("g++"):
+        pytest.skip("no g++")
+    src, exe = tmp_path / "layout.cpp", tmp_path / "layout"
+    src.write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", ROOT, str(src), "-o", str(exe)], check=True, timeout=120)
+    assert subprocess.run([str(exe)], timeout=60).returncode == 0
+
+
+def test_null_handles_are_refused():
+    lib, x = V.lib(), C.c_void_p(16)
+    assert V.KV_Q4_0 == 3
+    assert lib.vlrf_hip_kv_truncate(None, 0, 0) == _lib.ERR_ARG and "null cache" in _lib.last_error()
+    assert lib.vlrf_hip_attn_chunk(None, 0, x, x, 1, 1, 1, 1.0) == _lib.ERR_ARG and "null cache" in _lib.last_error()
+    h = C.c_void_p()
+    assert lib.vlrf_hip_kv_create(None, 1, 1, 1, 64, V.KV_Q4_0, C.byref(h)) == _lib.ERR_ARG and h.value is None

@@ -7,6 +7,7 @@ LIB_PATH = os.path.join(PKG, "libvlrf_hip.so")
 
 DT_F32, DT_Q4_0, DT_Q8_0 = 0, 2, 8
 KV_F32, KV_F16, KV_Q8_0 = 0, 1, 2     # KVCacheDType (kv_cache.hpp:37-41)
+KV_Q4_0 = 3                           # this library's own: Q4_0 blocks of 32 elements
 
 OK, ERR_ARG, ERR_RUNTIME, ERR_NOMEM, ERR_OVERFLOW, ERR_NODEV = 0, -1, -2, -3, -4, -5
 
@@ -49,10 +50,12 @@ _SIGS = {
     "vlrf_hip_kv_reset": (i32, [vp]),
     "vlrf_hip_kv_used": (i32, [vp, i32]),
     "vlrf_hip_kv_append": (i32, [vp, i32, vp, vp, i32]),
+    "vlrf_hip_kv_truncate": (i32, [vp, i32, i32]),
     "vlrf_hip_kv_read": (i32, [vp, i32, i32, i32, vp, vp, vp, vp]),
     "vlrf_hip_kv_dequant": (i32, [vp, i32, i32, vp, vp]),
     "vlrf_hip_attn_decode": (i32, [vp, i32, vp, vp, i32, i32, f32]),
     "vlrf_hip_attn_decode_noalloc": (i32, [vp, i32, vp, vp, i32, i32, f32]),
+    "vlrf_hip_attn_chunk": (i32, [vp, i32, vp, vp, i32, i32, i32, f32]),
     "vlrf_hip_weight_upload": (i32, [vp, vp, i32, i32, i32, C.POINTER(vp)]),
     "vlrf_hip_weight_free": (None, [vp]),
     "vlrf_hip_qgemm_plan": (i32, [i32, i32, i32, i32, i32, C.POINTER(C.c_int64)]),

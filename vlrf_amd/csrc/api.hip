@@ -247,10 +247,49 @@ struct vlrf_hip_kv {
     } while (0)
 
 namespace vlrf_hip {
+// The same of a Q4_0 cache: rows of GGUF blocks, put together from the codes and
+// scales of the groups of 32 keys that hold them.
+static int kv4_rows_to_host(hipStream_t s, const KVLayer& L, int G, int D, int max_seq, int row0, int n, int8_t* k_q,
+                            int8_t* v_q) {
+    if (!n) return VLRF_HIP_OK;
+    const int first = row0 / kv4::kKeys * kv4::kKeys, keys = (row0 + n - first + kv4::kKeys - 1) / kv4::kKeys * kv4::kKeys;
+    const int nb = D / 32;
+    std::vector<uint8_t> c;
+    std::vector<uint16_t> d;
+    try {
+        c.resize(kv4::head_codes(keys, D));
+        d.resize(kv4::head_scales(keys, D));
+    } catch (const std::bad_alloc&) {
+        set_error("kv_read: no host memory for %d rows", n);
+        return VLRF_HIP_ERR_NOMEM;
+    }
+    for (int g = 0; g < G; ++g)
+        for (const bool isv : {false, true}) {
+            int8_t* to = isv ? v_q : k_q;
+            if (!to) continue;
+            const int8_t* cs = (isv ? L.v : L.k) + g * kv4::head_codes(max_seq, D) + kv4::head_codes(first, D);
+            const uint16_t* ds = reinterpret_cast<const uint16_t*>(isv ? L.vs : L.ks) + g * kv4::head_scales(max_seq, D) +
+                                 kv4::head_scales(first, D);
+            VH_CHECK(hipMemcpyAsync(c.data(), cs, c.size(), hipMemcpyDeviceToHost, s));
+            VH_CHECK(hipMemcpyAsync(d.data(), ds, d.size() * 2, hipMemcpyDeviceToHost, s));
+            VH_CHECK(hipStreamSynchronize(s));
+            for (int r = 0; r < n; ++r)
+                for (int b = 0; b < nb; ++b) {
+                    const int t = row0 - first + r;
+                    int8_t* blk = to + (((size_t)r * G + g) * nb + b) * 18;
+                    std::memcpy(blk, &d[kv4::scale(t, b, D)], 2);
+                    for (int i = 0; i < 16; ++i)
+                        blk[2 + i] = (int8_t)c[isv ? kv4::v_byte(t, i, b, D) : kv4::k_word(t, i / 4, b, D) + i % 4];
+                }
+        }
+    return VLRF_HIP_OK;
+}
+
 // Rows [row0, row0+n) of a head-major cache layer to host, token-major, as
 // the cache's own elements (int8 codes, f16 bits or f32); scales for Q8_0.
 int kv_rows_to_host(hipStream_t s, const KVLayer& L, int G, int D, int max_seq, int row0, int n,
                     int8_t* k_q, int8_t* v_q, float* k_s, float* v_s) {
+    if (L.dtype == VLRF_HIP_KV_Q4_0) return kv4_rows_to_host(s, L, G, D, max_seq, row0, n, k_q, v_q);
     const size_t eb = (size_t)kv_elem_bytes(L.dtype), hd = (size_t)D * eb, row = (size_t)G * hd;
     std::vector<int8_t> hk((size_t)G * n * hd), hv((size_t)G * n * hd);
     for (int g = 0; g < G; ++g) {
@@ -458,11 +497,12 @@ int vlrf_hip_kv_create(vlrf_hip_ctx_t ctx, int n_layers, int max_seq, int n_kv_h
     VH_CTX(ctx);
     VH_ARG(out != nullptr, "kv_create: null output");
     *out = nullptr;
-    VH_ARG(dtype == VLRF_HIP_KV_Q8_0 || dtype == VLRF_HIP_KV_F16 || dtype == VLRF_HIP_KV_F32,
-           "kv_create: cache dtype %d is not F32, F16 or Q8_0", dtype);
+    VH_ARG(dtype == VLRF_HIP_KV_Q8_0 || dtype == VLRF_HIP_KV_F16 || dtype == VLRF_HIP_KV_F32 || dtype == VLRF_HIP_KV_Q4_0,
+           "kv_create: cache dtype %d is not F32, F16, Q8_0 or Q4_0", dtype);
     VH_ARG(n_layers >= 1 && max_seq >= 1 && n_kv_heads >= 1 && d_head >= 2 && d_head % 16 == 0,
            "kv_create: bad shape layers=%d max_seq=%d n_kv=%d d_head=%d", n_layers, max_seq,
            n_kv_heads, d_head);
+    VH_ARG(dtype != VLRF_HIP_KV_Q4_0 || d_head % 32 == 0, "kv_create: d_head %d is not whole Q4_0 blocks of 32", d_head);
     auto* kv = new (std::nothrow) vlrf_hip_kv();
     if (!kv) return VLRF_HIP_ERR_NOMEM;
     kv->ctx = ctx;
@@ -472,13 +512,12 @@ int vlrf_hip_kv_create(vlrf_hip_ctx_t ctx, int n_layers, int max_seq, int n_kv_h
     kv->d_head = d_head;
     kv->layers.resize(n_layers);
     kv->used.assign(n_layers, 0);
-    const size_t data = (size_t)n_kv_heads * max_seq * d_head * kv_elem_bytes(dtype);
+    const size_t data = kv_data_bytes(dtype, n_kv_heads, max_seq, d_head);
+    const size_t scales = kv_scale_bytes(dtype, n_kv_heads, max_seq, d_head);
     for (auto& L : kv->layers) {
         L.dtype = dtype;
-        const bool q8 = dtype == VLRF_HIP_KV_Q8_0;
         if (hipMalloc(&L.k, data) != hipSuccess || hipMalloc(&L.v, data) != hipSuccess ||
-            (q8 && hipMalloc(&L.ks, max_seq * sizeof(float)) != hipSuccess) ||
-            (q8 && hipMalloc(&L.vs, max_seq * sizeof(float)) != hipSuccess)) {
+            (scales && hipMalloc(&L.ks, scales) != hipSuccess) || (scales && hipMalloc(&L.vs, scales) != hipSuccess)) {
             vlrf_hip_kv_destroy(kv);
             set_error("kv_create: hipMalloc failed");
             return VLRF_HIP_ERR_NOMEM;
@@ -510,11 +549,12 @@ int vlrf_hip_kv_reset(vlrf_hip_kv_t kv) {
     VH_ARG(kv != nullptr, "kv_reset: null cache");
     VH_CTX(kv->ctx);
     for (auto& L : kv->layers) {
-        const size_t data = (size_t)kv->n_kv * kv->max_seq * kv->d_head * kv_elem_bytes(L.dtype);
+        const size_t data = kv_data_bytes(L.dtype, kv->n_kv, kv->max_seq, kv->d_head);
+        const size_t scales = kv_scale_bytes(L.dtype, kv->n_kv, kv->max_seq, kv->d_head);
         VH_CHECK(hipMemsetAsync(L.k, 0, data, kv->ctx->stream));
         VH_CHECK(hipMemsetAsync(L.v, 0, data, kv->ctx->stream));
-        if (L.ks) VH_CHECK(hipMemsetAsync(L.ks, 0, kv->max_seq * sizeof(float), kv->ctx->stream));
-        if (L.vs) VH_CHECK(hipMemsetAsync(L.vs, 0, kv->max_seq * sizeof(float), kv->ctx->stream));
+        if (L.ks) VH_CHECK(hipMemsetAsync(L.ks, 0, scales, kv->ctx->stream));
+        if (L.vs) VH_CHECK(hipMemsetAsync(L.vs, 0, scales, kv->ctx->stream));
     }
     VH_CHECK(hipStreamSynchronize(kv->ctx->stream));
     kv->used.assign(kv->n_layers, 0);
@@ -531,7 +571,7 @@ int vlrf_hip_kv_append(vlrf_hip_kv_t kv, int layer, const float* k, const float*
     VH_CTX(kv->ctx);
     VH_ARG(layer >= 0 && layer < kv->n_layers, "kv_append: layer %d out of range", layer);
     VH_ARG(k && v && T >= 1, "kv_append: bad arguments");
-    if (kv->used[layer] + T > kv->max_seq) {
+    if (T > kv->max_seq - kv->used[layer]) {
         set_error("KVCache::append: exceeds max_seq_len (%d + %d > %d)", kv->used[layer], T, kv->max_seq);
         return VLRF_HIP_ERR_OVERFLOW;
     }
@@ -542,6 +582,13 @@ int vlrf_hip_kv_append(vlrf_hip_kv_t kv, int layer, const float* k, const float*
     return VLRF_HIP_OK;
 }
 
+int vlrf_hip_kv_truncate(vlrf_hip_kv_t kv, int layer, int n) {
+    VH_ARG(kv != nullptr, "kv_truncate: null cache");
+    VH_ARG(layer >= 0 && layer < kv->n_layers, "kv_truncate: layer %d out of range", layer);
+    VH_ARG(n >= 0 && n <= kv->used[layer], "kv_truncate: %d rows of %d", n, kv->used[layer]);
+    kv->used[layer] = n;
+    return VLRF_HIP_OK;
+}
 
 int vlrf_hip_kv_read(vlrf_hip_kv_t kv, int layer, int row0, int n, int8_t* k_q, int8_t* v_q,
                      float* k_s, float* v_s) {
@@ -562,6 +609,25 @@ int vlrf_hip_kv_dequant(vlrf_hip_kv_t kv, int layer, int ctx_len, float* K_out, 
                              ctx_len, K_out, V_out);
 }
 
+// Attention of T rows over a Q4_0 cache (the arguments are checked by the callers).
+static int attn_kv4(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T, int ctx_len, float scale) {
+    return launch_attn_kv4(kv->ctx->stream, q, kv->layers[layer], n_heads, kv->n_kv, kv->d_head, kv->max_seq, T, ctx_len,
+                           scale, out);
+}
+
+int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T, int ctx_len,
+                        float scale) {
+    VH_ARG(kv != nullptr, "attn_chunk: null cache");
+    VH_CTX(kv->ctx);
+    VH_ARG(layer >= 0 && layer < kv->n_layers, "attn_chunk: layer %d out of range", layer);
+    VH_ARG(kv->layers[layer].dtype == VLRF_HIP_KV_Q4_0, "attn_chunk: the cache is not Q4_0 (dtype %d)",
+           kv->layers[layer].dtype);
+    VH_ARG(q && out && q != out, "attn_chunk: null or shared pointer");
+    VH_ARG(T >= 1 && T <= ctx_len && ctx_len <= kv->max_seq, "attn_chunk: %d rows of %d keys in a cache of %d", T, ctx_len,
+           kv->max_seq);
+    return attn_kv4(kv, layer, q, out, n_heads, T, ctx_len, scale);
+}
+
 int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads,
                          int ctx_len, float scale) {
     VH_ARG(kv != nullptr, "attn_decode: null cache");
@@ -570,6 +636,7 @@ int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out
     VH_ARG(q && out, "attn_decode: null pointer");
     VH_ARG(ctx_len >= 1 && ctx_len <= kv->max_seq, "attn_decode: ctx_len %d outside [1,%d]", ctx_len,
            kv->max_seq);
+    if (kv->layers[layer].dtype == VLRF_HIP_KV_Q4_0) return attn_kv4(kv, layer, q, out, n_heads, 1, ctx_len, scale);
     const int splits = attn_decode_splits(ctx_len);
     float* part = nullptr;
     int rc = kv->ctx->scratch((size_t)n_heads * splits * (kv->d_head + 2) * sizeof(float), &part);
@@ -596,6 +663,8 @@ int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, fl
            "attn_decode_noalloc: %zu partial floats (n_heads %d x %d splits x %d) exceed the fixed scratch of %zu",
            need, n_heads, splits, kv->d_head + 2, noalloc::kScratchFloats);
     const KVLayer& L = kv->layers[layer];
+    if (L.dtype == VLRF_HIP_KV_Q4_0)
+        return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out);
     return launch_attn_decode(kv->ctx->stream, q, L.k, L.v, L.ks, L.vs, L.dtype, (long)kv->max_seq * kv->d_head,
                               n_heads, kv->n_kv, kv->d_head, ctx_len, nullptr, splits, scale,
                               kv->ctx->noalloc_scratch, out, nullptr, kv->ctx->small_tile_ctr);

@@ -13,6 +13,7 @@
 #include <string>
 
 #include "../../include/vlrf_hip.h"
+#include "kernels/kv4_layout.hpp"
 
 namespace vlrf_hip {
 
@@ -105,17 +106,28 @@ bool weight_expand_bf16(hipStream_t s, const DevWeight& w);
 
 // ---- KV cache ------------------------------------------------------------------
 // k and v address [n_kv][max_seq][d_head] elements of the layer's dtype: int8
-// codes (Q8_0, with one f32 scale per token row in ks/vs), f16 bits or f32.
+// codes (Q8_0, with one f32 scale per token row in ks/vs), f16 bits or f32.  Q4_0:
+// packed codes in k/v and f16 scales in ks/vs, as kernels/kv4_layout.hpp orders them.
 struct KVLayer {
     int8_t* k = nullptr;
     int8_t* v = nullptr;
-    float* ks = nullptr;   // [max_seq], Q8_0 only
+    float* ks = nullptr;   // Q8_0 [max_seq] f32, Q4_0 f16
     float* vs = nullptr;
     int dtype = VLRF_HIP_KV_Q8_0;
 };
 
-__host__ __device__ inline int kv_elem_bytes(int dtype) {
+__host__ __device__ inline int kv_elem_bytes(int dtype) {   // not Q4_0
     return dtype == VLRF_HIP_KV_F32 ? 4 : dtype == VLRF_HIP_KV_F16 ? 2 : 1;
+}
+
+// Bytes of a layer's K (or V) elements and of their scales, any dtype.
+inline size_t kv_data_bytes(int dtype, int n_kv, int max_seq, int d) {
+    if (dtype == VLRF_HIP_KV_Q4_0) return n_kv * kv4::head_codes(max_seq, d);
+    return (size_t)n_kv * max_seq * d * kv_elem_bytes(dtype);
+}
+inline size_t kv_scale_bytes(int dtype, int n_kv, int max_seq, int d) {
+    if (dtype == VLRF_HIP_KV_Q4_0) return n_kv * kv4::head_scales(max_seq, d) * 2;
+    return dtype == VLRF_HIP_KV_Q8_0 ? max_seq * sizeof(float) : 0;
 }
 
 // KVCache's f32 -> f16 element conversion (kv_cache.hpp:68-97): the mantissa is
@@ -223,6 +235,15 @@ int launch_rope_append(hipStream_t s, const KVLayer& L, float* q, const float* k
                        const int* pos_dev, const float* cos_t, const float* sin_t);
 int launch_kv_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq,
                       int ctx_len, float* K_out, float* V_out);
+// The 4-bit cache (kernels/kv4.hip): rows [pos, pos + T) quantized from k/v
+// [T][n_kv*d_head], rows [0, ctx_len) read back, and the attention of T query rows
+// [T][n_heads*d_head], the last T of ctx_len tokens (row t sees ctx_len - T + t + 1 keys).
+int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, const float* k, const float* v,
+                      int T, int pos);
+int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, int ctx_len, float* K,
+                       float* V);
+int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
+                    int ctx_len, float scale, float* out);
 // Prefill: RoPE on k of T tokens of a [T][ld] QKV buffer at positions
 // pos0.., then the cache append of their K/V rows (q is left as it is: the
 // prefill attention rotates it as it loads it).

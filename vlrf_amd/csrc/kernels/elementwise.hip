@@ -507,6 +507,10 @@ __global__ __launch_bounds__(512) void argmax_pairs_step_kernel(const float2* __
 int launch_kv_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq,
                      const float* k, const float* v, int T, int pos, const int* pos_dev) {
     VH_ARG(T >= 1 && n_kv >= 1 && d_head >= 1, "kv_append: empty shape");
+    if (L.dtype == VLRF_HIP_KV_Q4_0) {
+        VH_ARG(!pos_dev, "kv_append: a Q4_0 cache takes its position from the host");
+        return launch_kv4_append(s, L, n_kv, d_head, max_seq, k, v, T, pos);
+    }
     if (!pos_dev) VH_ARG(pos >= 0 && pos + T <= max_seq, "kv_append: rows [%d,%d) beyond max_seq %d",
                          pos, pos + T, max_seq);
     hipLaunchKernelGGL(kv_append_kernel, dim3(T), dim3(256), 0, s, L.k, L.v, L.ks, L.vs, L.dtype, k, v, n_kv,
@@ -570,6 +574,7 @@ int launch_kv_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int
                       int ctx_len, float* K_out, float* V_out) {
     VH_ARG(ctx_len >= 0 && ctx_len <= max_seq, "kv_dequant: ctx_len %d outside [0,%d]", ctx_len, max_seq);
     if (ctx_len == 0) return VLRF_HIP_OK;
+    if (L.dtype == VLRF_HIP_KV_Q4_0) return launch_kv4_dequant(s, L, n_kv, d_head, max_seq, ctx_len, K_out, V_out);
     hipLaunchKernelGGL(kv_dequant_kernel, dim3(ctx_len), dim3(256), 0, s, L.k, L.v, L.ks, L.vs, L.dtype, n_kv,
                        d_head, max_seq, K_out, V_out);
     VH_LAUNCHED();

@@ -7,7 +7,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import lib, check, ModelConfig, DT_F32, KV_F16, KV_F32, KV_Q8_0
+from ._lib import lib, check, ModelConfig, DT_F32, KV_F16, KV_F32, KV_Q4_0, KV_Q8_0
 
 
 class DeviceBuffer:
@@ -170,7 +170,8 @@ class QuantWeight:
 
 
 class KVCache:
-    """Device Q8_0 KV cache for n_layers (KVCache, kv_cache.hpp:132-293)."""
+    """Device KV cache for n_layers (KVCache, kv_cache.hpp:132-293), Q8_0 unless
+    `dtype` says otherwise; KV_Q4_0 needs d_head a multiple of 32."""
 
     def __init__(self, ctx, n_layers, max_seq_len, n_kv_heads, d_head, dtype=KV_Q8_0):
         self.ctx = ctx
@@ -192,10 +193,19 @@ class KVCache:
     def append(self, layer, k, v, T):
         check(lib().vlrf_hip_kv_append(self.h, layer, k.ptr, v.ptr, T))
 
+    def truncate(self, layer, n):
+        """Forgets the rows from n on; appends go on there."""
+        check(lib().vlrf_hip_kv_truncate(self.h, layer, n))
+
     def read(self, layer, row0, n):
         """(K [n,row], V [n,row], K scales [n], V scales [n]) in the reference's
         token-major layout: int8 codes with f32 scales (Q8_0), or uint16 f16
-        bits / float32 elements with the scales None."""
+        bits / float32 elements with the scales None; KV_Q4_0: uint8 [n, row/32, 18]
+        blocks (formats.dequantize reads them), the scales None."""
+        if self.dtype == KV_Q4_0:
+            kb, vb = (np.zeros((n, self.row_dim // 32, 18), np.uint8) for _ in range(2))
+            check(lib().vlrf_hip_kv_read(self.h, layer, row0, n, kb.ctypes.data, vb.ctypes.data, None, None))
+            return kb, vb, None, None
         et = {KV_F32: np.float32, KV_F16: np.uint16}.get(self.dtype, np.int8)
         kq = np.zeros((n, self.row_dim), et)
         vq = np.zeros((n, self.row_dim), et)
@@ -212,6 +222,11 @@ class KVCache:
     def attention_decode(self, layer, q, out, n_heads, ctx_len, scale):
         check(lib().vlrf_hip_attn_decode(self.h, layer, q.ptr, out.ptr, n_heads, ctx_len,
                                          float(scale)))
+
+    def attention_chunk(self, layer, q, out, n_heads, T, ctx_len, scale):
+        """Causal attention of T query rows (device [T, n_heads*d_head]), the last T
+        of ctx_len tokens, over a KV_Q4_0 cache."""
+        check(lib().vlrf_hip_attn_chunk(self.h, layer, q.ptr, out.ptr, n_heads, T, ctx_len, float(scale)))
 
     def __del__(self):
         try:
