@@ -21,9 +21,11 @@ from vlrf_amd import formats as F
 pytestmark = pytest.mark.gpu
 
 
-def _attention64(q, K, Vv, n_heads, scale):
-    """(result [T, H, d], bound) for q [T, H, d] and the cache's values K, Vv [n, G, d]."""
+def _attention64(q, K, Vv, n_heads, scale, terms=None):
+    """(result [T, H, d], bound) for q [T, H, d] and the cache's values K, Vv [n, G, d]; terms: the
+    products that a score adds up where they are fewer than d."""
     T, _, d = q.shape
+    terms = terms or d
     n, G, _ = K.shape
     q, K, Vv = (t.astype(np.float64) for t in (q, K, Vv))
     keep = np.arange(n)[None, :] <= np.arange(T)[:, None] + (n - T)
@@ -36,7 +38,7 @@ def _attention64(q, K, Vv, n_heads, scale):
         p /= L
         S = np.where(keep, np.abs(q[:, h]) @ np.abs(k).T * abs(scale), 0).max(1, keepdims=True)
         out[:, h] = p @ v
-        bound[:, h] = 2 * 2.0 ** -24 * ((d + 16) * S + n + 64) * (p @ np.abs(v)) + n * 2.0 ** -31 / L
+        bound[:, h] = 2 * 2.0 ** -24 * ((terms + 16) * S + n + 64) * (p @ np.abs(v)) + n * 2.0 ** -31 / L
     return out, bound
 
 
@@ -240,6 +242,22 @@ def test_ranges_of_queries(ctx):
     bad[5, 2] = bad[6, 3] = True
     assert np.isnan(got[bad]).all()
     assert (np.abs(got - ref) <= bound)[~bad].all()
+
+
+@pytest.mark.parametrize("G,rep,d,T", [(64, 8, 64, 3), (128, 1, 128, 2), (16, 16, 128, 60)])
+def test_pieces_add_up(ctx, G, rep, d, T):
+    """Queries with one element that is not zero, few keys: nothing but the two pieces of q and of the
+    weights rounds, and a piece that does not fit the other (2^-11 off) stands out."""
+    print(f"[case] kv4 pieces G={G} rep={rep} d={d} T={T}", flush=True)
+    H = G * rep
+    kv, K, Vv = _filled(ctx, T, G, d, 99)
+    q = np.zeros((T, H, d), np.float32)
+    at = np.arange(T * H)
+    q.reshape(T * H, d)[at, at * 7 % d] = F.normal(99, "q", T * H, 4.0)
+    out = ctx.alloc(q.nbytes)
+    kv.attention_chunk(0, ctx.to_device(q), out, H, T, T, 1.0)
+    ref, bound = _attention64(q, K, Vv, H, np.float32(1.0), terms=1)
+    assert (np.abs(out.download(q.shape) - ref) <= bound).all()
 
 
 def test_one_token_is_the_decode_call(ctx):

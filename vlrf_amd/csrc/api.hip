@@ -611,8 +611,14 @@ int vlrf_hip_kv_dequant(vlrf_hip_kv_t kv, int layer, int ctx_len, float* K_out, 
 
 // Attention of T rows over a Q4_0 cache (the arguments are checked by the callers).
 static int attn_kv4(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T, int ctx_len, float scale) {
+    float* part = nullptr;
+    const size_t need = attn_kv4_part_bytes(n_heads, kv->n_kv, kv->d_head, T, ctx_len);
+    if (need) {
+        const int rc = kv->ctx->scratch(need, &part);
+        if (rc) return rc;
+    }
     return launch_attn_kv4(kv->ctx->stream, q, kv->layers[layer], n_heads, kv->n_kv, kv->d_head, kv->max_seq, T, ctx_len,
-                           scale, out);
+                           scale, out, part);
 }
 
 int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T, int ctx_len,
@@ -664,7 +670,8 @@ int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, fl
            need, n_heads, splits, kv->d_head + 2, noalloc::kScratchFloats);
     const KVLayer& L = kv->layers[layer];
     if (L.dtype == VLRF_HIP_KV_Q4_0)
-        return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out);
+        return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out,
+                               kv->ctx->noalloc_scratch);
     return launch_attn_decode(kv->ctx->stream, q, L.k, L.v, L.ks, L.vs, L.dtype, (long)kv->max_seq * kv->d_head,
                               n_heads, kv->n_kv, kv->d_head, ctx_len, nullptr, splits, scale,
                               kv->ctx->noalloc_scratch, out, nullptr, kv->ctx->small_tile_ctr);

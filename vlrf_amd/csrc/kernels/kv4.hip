@@ -10,6 +10,7 @@
 #include "kv4_layout.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace vlrf_hip {
 namespace {
@@ -80,52 +81,390 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
     reinterpret_cast<float2*>(V)[i] = make_float2((float)((int)(vb & 15u) - 8) * vd, (float)((int)(vb >> 4) - 8) * vd);
 }
 
-// One workgroup a query row of one head; its four waves take the keys in turn, lane
-// l elements 2l and 2l + 1 (d 64: half of the lanes idle), each wave with its own
-// running maximum and sum, merged at the end.
-template <int D>
-__global__ __launch_bounds__(256) void kv4_attn_row_kernel(const float* __restrict__ q, const uint8_t* __restrict__ kc,
-                                                           const uint8_t* __restrict__ vc,
-                                                           const uint16_t* __restrict__ ks,
-                                                           const uint16_t* __restrict__ vs, int n_heads, int rep,
-                                                           int max_seq, int T, int ctx, float scale,
-                                                           float* __restrict__ out) {
-    __shared__ float wm[4], wl[4], wo[4][D];
-    const int h = blockIdx.x % n_heads, t = blockIdx.x / n_heads, g = h / rep;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, p = lane % (D / 2), b = p / 16, l = p % 16;
-    const bool on = lane < D / 2;
-    const int seen = ctx - T + t + 1;
-    const size_t row = ((size_t)t * n_heads + h) * D;
-    const float q0 = on ? q[row + 2 * p] : 0.f, q1 = on ? q[row + 2 * p + 1] : 0.f;
-    kc += g * kv4::head_codes(max_seq, D);
-    vc += g * kv4::head_codes(max_seq, D);
-    ks += g * kv4::head_scales(max_seq, D);
-    vs += g * kv4::head_scales(max_seq, D);
-    float m = kNegInf, sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j = w; j < seen; j += 4) {
-        const size_t si = kv4::scale(j, b, D);
-        const uint32_t kb = kc[kv4::k_word(j, l / 4, b, D) + l % 4], vb = vc[kv4::v_byte(j, l, b, D)];
-        const float kd = f16_bits_to_f32(ks[si]), vd = f16_bits_to_f32(vs[si]);
-        const float dot = on ? (q0 * (float)((int)(kb & 15u) - 8) + q1 * (float)((int)(kb >> 4) - 8)) * kd : 0.f;
-        const float s = wave_sum(dot) * scale, mn = fmaxf(m, s);
-        const float c = m == kNegInf ? 0.f : expf(m - mn), e = expf(mn == kNegInf ? s : s - mn);   // a NaN score stays
-        sum = sum * c + e;
-        o0 = o0 * c + e * ((float)((int)(vb & 15u) - 8) * vd);
-        o1 = o1 * c + e * ((float)((int)(vb >> 4) - 8) * vd);
-        m = mn;
+// ---- attention --------------------------------------------------------------------
+// The T * rep query rows of a KV head (rep query heads share it) stand as rows t rep
+// + r, 16 NG of them a workgroup; its four waves take the chunk's groups of 32 keys
+// in turn, each with its own running maximum and sum, and merge through LDS.
+//   scores   S^T = K Q^T, 16 keys by 16 rows and a block of 32 elements an
+//            instruction.  A code minus 8 is exact in f16; q, scaled by a power of
+//            two for the row's largest element to lie in [2^13, 2^14), enters as two
+//            f16 pieces (22 bits).  Each block's sum is scaled in f32.
+//   weights  p = 2^(s - m + 10).  m moves when a score passes it by 4 (in powers of
+//            two), so p <= 2^14; rescaling O is rare and skipped by the wave.
+//   output   O^T = V^T P^T over the same codes: p times the key's scale, in two f16
+//            pieces, is the other operand.  It stays below 2^15 while scales are
+//            below 2; a block with a larger one among the 32 keys' has its products
+//            formed apart, scaled down by a power of two, and added scaled up.
+// A lane's scores are of the row that is its column in both products and of the keys
+// that its group of V's layout holds, so nothing moves between lanes but the
+// maximum's two exchanges a group.
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+constexpr float kHeadroom = 4.f, kWeightBits = 10.f;
+constexpr int kWaves = 4;
+
+struct Kv4Attn {
+    const float* q;          // [T][n_heads][D]
+    const uint8_t *kc, *vc;  // the layer's codes and scales
+    const uint16_t *ks, *vs;
+    float *out, *part;       // [T][n_heads][D]; [T][n_heads][nch][D + 2] where nch > 1
+    size_t codes, scales;    // of a head
+    int n_heads, n_kv, rep, T, ctx;
+    int rounds, nch;         // groups of 32 keys a wave takes, chunks of the context
+    float sl2, qsign;        // |scale| log2(e), the scale's sign
+};
+
+__device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
+
+// The eight codes of a word, minus 8, as f16.  0x6400 | n is 1024 + n; with n four
+// bits higher 1024 + 16 n.  SHIFT 0: nibbles 0, 4, 1, 5, 2, 6, 3, 7 of the word.
+__device__ __forceinline__ void codes8(uint32_t w, h2v& a, h2v& b, h2v& c, h2v& d) {
+    const h2v low = {(_Float16)1032.f, (_Float16)1032.f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
+              high = {(_Float16)-72.f, (_Float16)-72.f};
+    const uint32_t u = w >> 8;
+    a = as_h2((w & 0x000F000Fu) | 0x64006400u) - low;
+    b = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+    c = as_h2((u & 0x000F000Fu) | 0x64006400u) - low;
+    d = __builtin_elementwise_fma(as_h2((u & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+}
+
+__device__ __forceinline__ h8v h8_of(h2v a, h2v b, h2v c, h2v d) { return h8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
+
+// Two f16 pieces of eight values.  The values are products: where the compiler fuses
+// one of them into a conversion, it rounds once instead of twice, and the piece that
+// is subtracted may not be the one that is multiplied; the empty asm keeps it from it.
+__device__ __forceinline__ void split8(float (&x)[8], h8v& hi, h8v& lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        asm("" : "+v"(x[e]));
+        hi[e] = (_Float16)x[e];
+        lo[e] = (_Float16)(x[e] - (float)hi[e]);
     }
-    if (lane == 0) { wm[w] = m; wl[w] = sum; }
-    if (on) { wo[w][2 * p] = o0; wo[w][2 * p + 1] = o1; }
+}
+
+__device__ __forceinline__ float over_groups_max(float v) {   // over the lanes of a column
+    float2 t = swap_rows16(v, v);
+    v = fmaxf(t.x, t.y);
+    t = swap_halves32(v, v);
+    return fmaxf(t.x, t.y);
+}
+
+__device__ __forceinline__ float over_groups_sum(float v) {
+    float2 t = swap_rows16(v, v);
+    v = t.x + t.y;
+    t = swap_halves32(v, v);
+    return t.x + t.y;
+}
+
+// A wave's share of 32 keys as it is loaded: lane (c, L) holds K words of keys c and
+// 16 + c, V bytes of elements 2c, 2c + 1 of each block for the keys of group L, and
+// those keys' scales.
+template <int NB>
+struct Kv4Raw {
+    uint32_t k[2][NB], v[2 * NB];
+    uint4 ks[NB], vs[NB];
+};
+
+template <int NB>
+__device__ __forceinline__ void kv4_load(Kv4Raw<NB>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks,
+                                         const uint16_t* vs, int kb, int c, int L) {
+    constexpr int D = 32 * NB;
+    const uint8_t* kp = kc + (size_t)kb * (kv4::kKeys * D / 2) + c * (D / 2) + 4 * L * NB;
+    const uint8_t* vp = vc + (size_t)kb * (kv4::kKeys * D / 2) + (L * 16 + c) * (8 * NB);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) __builtin_memcpy(r.k[u], __builtin_assume_aligned(kp + u * 16 * (D / 2), 4 * NB), 4 * NB);
+    const uint4* kq = reinterpret_cast<const uint4*>(ks + (size_t)kb * D) + L * NB;
+    const uint4* vq = reinterpret_cast<const uint4*>(vs + (size_t)kb * D) + L * NB;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) r.ks[b] = kq[b];
+    __builtin_memcpy(r.v, __builtin_assume_aligned(vp, 8 * NB), 8 * NB);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) r.vs[b] = vq[b];
+}
+
+// Slots 2j and 2j + 1 of a lane's eight scales.
+__device__ __forceinline__ uint32_t word_of(const uint4& x, int j) { return j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w; }
+
+template <int D, int NG>
+__global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_kernel(Kv4Attn a) {
+    constexpr int NB = D / 32, ROWS = 16 * NG, OS = D + 4;
+    __shared__ __align__(16) float os[kWaves][ROWS * OS];
+    __shared__ float ms[kWaves][ROWS], ls[kWaves][ROWS];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
+    const int nch = a.nch, chunk = blockIdx.x % nch, blk = blockIdx.x / nch;
+    const int g = blk % a.n_kv, row0 = blk / a.n_kv * ROWS, R = a.T * a.rep;
+    const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
+    const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
+    auto q_row = [&](int row) {   // of the T * n_heads rows of q
+        const int t = row / a.rep;
+        return (size_t)t * a.n_heads + g * a.rep + (row - t * a.rep);
+    };
+    // Keys that the block's first and last row see; the lane's rows' own.
+    const int past = a.ctx - a.T + 1;
+    const int fewest = past + row0 / a.rep, most = past + min(row0 + ROWS - 1, R - 1) / a.rep;
+    const int kb0 = chunk * kWaves * a.rounds + w;
+    const int mine = min(a.rounds, max(0, ((most + kv4::kKeys - 1) / kv4::kKeys - kb0 + kWaves - 1) / kWaves));
+
+    Kv4Raw<NB> raw;
+    if (mine > 0) kv4_load<NB>(raw, kc, vc, ks, vs, kb0, c, L);
+
+    h8v qh[NG][NB], ql[NG][NB];
+    float factor[NG], m2[NG], l[NG];
+    int seen[NG];
+    f4v o[NG][2 * NB];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const int row = min(row0 + 16 * n + c, R - 1);
+        const float* qp = a.q + q_row(row) * D + 8 * L;
+        float x[NB][8], amax = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float y[8];
+            __builtin_memcpy(y, qp + 32 * b, 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[e];   // in the order of codes8
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
+        }
+        amax = over_groups_max(amax);
+        const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 120);
+        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+        factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[b][e] *= up;
+            split8(x[b], qh[n][b], ql[n][b]);
+        }
+        seen[n] = past + row / a.rep;
+        m2[n] = kNegInf;
+        l[n] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) o[n][t] = f4v{};
+    }
+
+    // One group of 32 keys.  CAREFUL: some row does not see all of them, or a value
+    // block's scale is 2 or more (or no number).
+    auto group = [&](auto careful, const Kv4Raw<NB>& cur, int key0) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        // ---- scores: slots 4u + j of the lane's keys ----
+        float s[NG][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                h2v k0, k1, k2, k3;
+                codes8(cur.k[u][b], k0, k1, k2, k3);
+                const h8v ka = h8_of(k0, k1, k2, k3);
+                const h2v d0 = as_h2(word_of(cur.ks[b], 2 * u)), d1 = as_h2(word_of(cur.ks[b], 2 * u + 1));
+                const float dk[4] = {(float)d0.x, (float)d0.y, (float)d1.x, (float)d1.y};
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {
+                    f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], f4v{}, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], t, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[n][4 * u + j] = b == 0 ? t[j] * dk[j] : fmaf(t[j], dk[j], s[n][4 * u + j]);
+                }
+            }
+
+        // ---- softmax ----
+        auto hidden = [&](int n, int e) { return key0 + kv4::key_of(L, e) >= seen[n]; };
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            if constexpr (CAREFUL) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[n][e] = hidden(n, e) ? kNegInf : s[n][e];
+            }
+            float mx = s[n][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[n][e]);
+            mx = over_groups_max(mx);
+            mx = mx == kNegInf ? kNegInf : mx * factor[n];
+            const bool grow = mx > m2[n] + kHeadroom;
+            const float mn = grow ? mx : m2[n];
+            const float corr = grow ? __builtin_amdgcn_exp2f(m2[n] - mn) : 1.f;
+            m2[n] = mn;
+            const float at = mn == kNegInf ? 0.f : kWeightBits - mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float p = __builtin_amdgcn_exp2f(fmaf(s[n][e], factor[n], at));
+                if constexpr (CAREFUL) p = hidden(n, e) ? 0.f : p;
+                s[n][e] = p;
+                sum += p;
+            }
+            l[n] = fmaf(l[n], corr, sum);
+            if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+                for (int t = 0; t < 2 * NB; ++t) o[n][t] *= corr;
+            }
+        }
+
+        // ---- output ----
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            h2v v0, v1, v2, v3, w0, w1, w2, w3;
+            codes8(cur.v[2 * b], v0, w0, v1, w1);        // slots 0, 2 and 1, 3: even elements, odd elements
+            codes8(cur.v[2 * b + 1], v2, w2, v3, w3);    // slots 4, 6 and 5, 7
+            const h8v va = h8_of(v0, v1, v2, v3), wa = h8_of(w0, w1, w2, w3);
+            int down = 0;                                // powers of two that the block's products are formed below
+            if constexpr (CAREFUL) {
+                uint32_t top = 15;                       // the largest exponent of the finite scales
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t x = (word_of(cur.vs[b], j >> 1) >> (16 * (j & 1) + 10)) & 31u;
+                    top = x < 31u ? max(top, x) : top;
+                }
+                down = (int)over_groups_max((float)top) - 15;
+            }
+            const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const h2v d = as_h2(word_of(cur.vs[b], e >> 1));
+                    const int to = (e & 4) + 2 * (e & 1) + ((e >> 1) & 1);
+                    x[to] = (CAREFUL ? s[n][e] * scale_down : s[n][e]) * (float)((e & 1) ? d.y : d.x);
+                    if constexpr (CAREFUL) x[to] = hidden(n, e) ? 0.f : x[to];   // whatever the scale is
+                }
+                h8v ph, pl;
+                split8(x, ph, pl);
+                if (!CAREFUL || __builtin_amdgcn_readfirstlane(down) == 0) {
+                    o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, o[n][2 * b], 0, 0, 0);
+                    o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, o[n][2 * b + 1], 0, 0, 0);
+                    o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, o[n][2 * b], 0, 0, 0);
+                    o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, o[n][2 * b + 1], 0, 0, 0);
+                } else {
+                    const float back = __uint_as_float((uint32_t)(127 + down) << 23);
+                    f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, f4v{}, 0, 0, 0);
+                    f4v z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, f4v{}, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, t, 0, 0, 0);
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, z, 0, 0, 0);
+                    o[n][2 * b] += t * back;
+                    o[n][2 * b + 1] += z * back;
+                }
+            }
+        }
+    };
+    for (int i = 0; i < mine; ++i) {
+        const int kb = kb0 + i * kWaves, key0 = kb * kv4::kKeys;
+        const Kv4Raw<NB> cur = raw;
+        if (i + 1 < mine) kv4_load<NB>(raw, kc, vc, ks, vs, kb + kWaves, c, L);
+        uint32_t large = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) large |= cur.vs[b].x | cur.vs[b].y | cur.vs[b].z | cur.vs[b].w;
+        if (key0 + kv4::kKeys > fewest || __builtin_amdgcn_ballot_w64((large & 0x40004000u) != 0)) group(std::true_type(), cur, key0);
+        else group(std::false_type(), cur, key0);
+    }
+
+    // ---- the waves' results, then the chunk's ----
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const float sum = over_groups_sum(l[n]);
+        if (L == 0) {
+            ms[w][16 * n + c] = sum != sum ? INFINITY : m2[n];   // a NaN has to win where the others' weights would drop it
+            ls[w][16 * n + c] = sum;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)   // rows 4L + j of the two tiles: elements 8L + 2j and 8L + 2j + 1 of the block
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float4*>(&os[w][(16 * n + c) * OS + 32 * b + 8 * L + 4 * h]) =
+                    make_float4(o[n][2 * b][2 * h], o[n][2 * b + 1][2 * h], o[n][2 * b][2 * h + 1], o[n][2 * b + 1][2 * h + 1]);
+    }
     __syncthreads();
-    if (threadIdx.x >= D) return;
-    float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3])), S = 0.f, O = 0.f;
-    for (int i = 0; i < 4; ++i) {
-        if (wm[i] == kNegInf && wl[i] == 0.f) continue;   // a wave without keys
-        const float f = wm[i] == kNegInf ? 1.f : expf(wm[i] - M);
-        S += f * wl[i];
-        O += f * wo[i][threadIdx.x];
+    const int rows = min(ROWS, R - row0);
+    for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) {
+        const int r = i / D, e = i - r * D;
+        float M = ms[0][r], sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) M = fmaxf(M, ms[k][r]);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float f = ms[k][r] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms[k][r] - M);
+            sum += f * ls[k][r];
+            x += f * os[k][r * OS + e];
+        }
+        const size_t at = q_row(row0 + r);
+        if (nch == 1) {
+            a.out[at * D + e] = sum == 0.f ? 0.f : x / sum;
+        } else {
+            float* p = a.part + (at * nch + chunk) * (D + 2);
+            p[e] = x;
+            if (e == 0) {
+                p[D] = M;
+                p[D + 1] = sum;
+            }
+        }
     }
-    out[row + threadIdx.x] = S == 0.f ? 0.f : O / S;
+}
+
+// out[row] = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the row's chunks.  W
+// waves a row (eight a workgroup), wave w's chunks w, w + W, ..., eight at a time
+// whose loads are all issued before any is used; the waves merge through LDS.
+template <int D, int W>
+__global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, int rows,
+                                                        float* __restrict__ out) {
+    constexpr int B = 8, V = D / 64;
+    __shared__ float sm[8], sl[8], so[8][D];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
+    const int row = (int)blockIdx.x * (8 / W) + wave / W;
+    float M = kNegInf, sum = 0.f, o[V] = {};
+    if (row < rows) {
+        const float* p = part + (size_t)row * nch * (D + 2);
+        for (int c0 = w; c0 < nch; c0 += B * W) {
+            float pm[B], pl[B], po[B][V], mb = M;
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const float* pc = p + (size_t)min(c0 + b * W, nch - 1) * (D + 2);
+                pm[b] = pc[D];
+                pl[b] = pc[D + 1];
+                __builtin_memcpy(po[b], __builtin_assume_aligned(pc + V * lane, 4 * V), 4 * V);
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
+            const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+            sum *= f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] *= f;
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const bool on = c0 + b * W < nch && pm[b] != kNegInf;   // an empty chunk has no accumulators
+                const float e = on ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
+                sum += on ? e * pl[b] : 0.f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] += on ? e * po[b][v] : 0.f;
+            }
+            M = mb;
+        }
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) { sm[wave] = M; sl[wave] = sum; }
+#pragma unroll
+        for (int v = 0; v < V; ++v) so[wave][V * lane + v] = o[v];
+        __syncthreads();
+        if (w) return;
+        const float m0 = M;
+#pragma unroll
+        for (int k = 1; k < W; ++k) M = fmaxf(M, sm[wave + k]);
+        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+        sum *= f0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= f0;
+#pragma unroll
+        for (int k = 1; k < W; ++k) {
+            const float f = sm[wave + k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sm[wave + k] - M);
+            sum += f * sl[wave + k];
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += f * so[wave + k][V * lane + v];
+        }
+    }
+    if (row >= rows) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[(size_t)row * D + V * lane + v] = sum == 0.f ? 0.f : o[v] / sum;
 }
 
 }  // namespace
@@ -154,20 +493,83 @@ int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, in
     return VLRF_HIP_OK;
 }
 
+namespace {
+// Workgroups of a launch: ROWS rows a block, `rounds` groups of 32 keys a wave.
+struct Kv4Plan {
+    int groups = 1, blocks = 1, rounds = 1, nch = 1;   // 16-row groups a block, blocks (KV heads included)
+};
+
+Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
+    Kv4Plan p;
+    const long R = (long)T * (n_heads / n_kv);
+    p.groups = R > 16 ? 2 : 1;
+    p.blocks = (int)((R + 16 * p.groups - 1) / (16 * p.groups)) * n_kv;
+    const long nb = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
+    const long want = 512;
+    p.rounds = (int)((nb * p.blocks + kWaves * want - 1) / (kWaves * want));
+    p.nch = (int)((nb + kWaves * p.rounds - 1) / (kWaves * p.rounds));
+    return p;
+}
+}  // namespace
+
+size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
+    if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1) return 0;   // refused by the launch
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    return p.nch > 1 ? (size_t)T * n_heads * p.nch * (d_head + 2) * sizeof(float) : 0;
+}
+
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
-                    int ctx_len, float scale, float* out) {
+                    int ctx_len, float scale, float* out, float* part) {
     VH_ARG(n_kv >= 1 && n_heads >= 1 && n_heads % n_kv == 0, "attn: n_heads %d not a multiple of n_kv %d", n_heads, n_kv);
     VH_ARG(d_head == 64 || d_head == 128, "attn: d_head %d not in {64,128}", d_head);
     VH_ARG(ctx_len >= 1 && ctx_len <= max_seq && T >= 1 && T <= ctx_len, "attn: %d rows of %d keys in a cache of %d", T,
            ctx_len, max_seq);
-    const dim3 grid((unsigned)((size_t)T * n_heads));
-#define VH_ROW(D)                                                                                                     \
-    VH_LAUNCH(kv4_attn_row_kernel<D>, grid, dim3(256), 0, s, q, reinterpret_cast<const uint8_t*>(L.k),                \
-              reinterpret_cast<const uint8_t*>(L.v), reinterpret_cast<const uint16_t*>(L.ks),                         \
-              reinterpret_cast<const uint16_t*>(L.vs), n_heads, n_heads / n_kv, max_seq, T, ctx_len, scale, out)
-    if (d_head == 64) VH_ROW(64);
-    else VH_ROW(128);
-#undef VH_ROW
+    VH_ARG((long)T * n_heads < (1l << 31), "attn: %d rows of %d heads", T, n_heads);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    VH_ARG((long)p.blocks * p.nch < (1l << 31), "attn: %d rows of %d heads over %d keys", T, n_heads, ctx_len);
+    VH_ARG(p.nch == 1 || part, "attn: no scratch");
+    Kv4Attn a;
+    a.q = q;
+    a.kc = reinterpret_cast<const uint8_t*>(L.k);
+    a.vc = reinterpret_cast<const uint8_t*>(L.v);
+    a.ks = reinterpret_cast<const uint16_t*>(L.ks);
+    a.vs = reinterpret_cast<const uint16_t*>(L.vs);
+    a.out = out;
+    a.part = part;
+    a.codes = kv4::head_codes(max_seq, d_head);
+    a.scales = kv4::head_scales(max_seq, d_head);
+    a.n_heads = n_heads;
+    a.n_kv = n_kv;
+    a.rep = n_heads / n_kv;
+    a.T = T;
+    a.ctx = ctx_len;
+    a.rounds = p.rounds;
+    a.nch = p.nch;
+    a.sl2 = (float)(std::fabs((double)scale) * 1.4426950408889634);
+    a.qsign = scale < 0.f ? -1.f : 1.f;
+    const dim3 grid((unsigned)((long)p.blocks * p.nch));
+#define VH_ROWS(D, G) VH_LAUNCH((kv4_attn_rows_kernel<D, G>), grid, dim3(64 * kWaves), 0, s, a)
+    if (d_head == 64) {
+        if (p.groups == 1) VH_ROWS(64, 1);
+        else VH_ROWS(64, 2);
+    } else {
+        if (p.groups == 1) VH_ROWS(128, 1);
+        else VH_ROWS(128, 2);
+    }
+#undef VH_ROWS
+    VH_LAUNCHED();
+    if (p.nch == 1) return VLRF_HIP_OK;
+    const int rows = T * n_heads;
+#define VH_MERGE(D, W) \
+    VH_LAUNCH((kv4_merge_kernel<D, W>), dim3((rows + 8 / W - 1) / (8 / W)), dim3(512), 0, s, part, p.nch, rows, out)
+    if (d_head == 64) {
+        if (p.nch <= 8) VH_MERGE(64, 1);
+        else VH_MERGE(64, 8);
+    } else {
+        if (p.nch <= 8) VH_MERGE(128, 1);
+        else VH_MERGE(128, 8);
+    }
+#undef VH_MERGE
     VH_LAUNCHED();
     return VLRF_HIP_OK;
 }
