@@ -118,30 +118,36 @@ struct Kv4Attn {
 
 __device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
 
-// The eight codes of a word, minus 8, as f16.  0x6400 | n is 1024 + n; with n four
-// bits higher 1024 + 16 n.  SHIFT 0: nibbles 0, 4, 1, 5, 2, 6, 3, 7 of the word.
-__device__ __forceinline__ void codes8(uint32_t w, h2v& a, h2v& b, h2v& c, h2v& d) {
+// 0x6400 twice, in a vector register: v_and_or_b32 takes no literal and one scalar.
+__device__ __forceinline__ uint32_t magic1024() {
+    uint32_t m = 0x64006400u;
+    asm("" : "+v"(m));
+    return m;
+}
+
+// The eight codes of a word, minus 8, as f16: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+// 0x6400 | n is 1024 + n; with n four bits higher 1024 + 16 n.
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t magic, h2v& a, h2v& b, h2v& c, h2v& d) {
     const h2v low = {(_Float16)1032.f, (_Float16)1032.f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
               high = {(_Float16)-72.f, (_Float16)-72.f};
     const uint32_t u = w >> 8;
-    a = as_h2((w & 0x000F000Fu) | 0x64006400u) - low;
-    b = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-    c = as_h2((u & 0x000F000Fu) | 0x64006400u) - low;
-    d = __builtin_elementwise_fma(as_h2((u & 0x00F000F0u) | 0x64006400u), sixteenth, high);
+    a = as_h2((w & 0x000F000Fu) | magic) - low;
+    b = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | magic), sixteenth, high);
+    c = as_h2((u & 0x000F000Fu) | magic) - low;
+    d = __builtin_elementwise_fma(as_h2((u & 0x00F000F0u) | magic), sixteenth, high);
 }
 
 __device__ __forceinline__ h8v h8_of(h2v a, h2v b, h2v c, h2v d) { return h8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
 
-// Two f16 pieces of eight values.  The values are products: where the compiler fuses
-// one of them into a conversion, it rounds once instead of twice, and the piece that
-// is subtracted may not be the one that is multiplied; the empty asm keeps it from it.
-__device__ __forceinline__ void split8(float (&x)[8], h8v& hi, h8v& lo) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        asm("" : "+v"(x[e]));
-        hi[e] = (_Float16)x[e];
-        lo[e] = (_Float16)(x[e] - (float)hi[e]);
-    }
+// Two f16 pieces of the products x f and y g: together 22 bits.  The first ones pass
+// through an empty asm, so that the piece that is subtracted is the one that is
+// multiplied: the compiler would form it twice, by a conversion of the rounded
+// product and by one that is fused with the product, which now and then differ.
+__device__ __forceinline__ void split2(float x, float f, float y, float g, h2v& hi, h2v& lo) {
+    uint32_t h = __builtin_bit_cast(uint32_t, h2v{(_Float16)fmaf(x, f, 0.f), (_Float16)fmaf(y, g, 0.f)});
+    asm("" : "+v"(h));
+    hi = as_h2(h);
+    lo = h2v{(_Float16)fmaf(x, f, -(float)hi.x), (_Float16)fmaf(y, g, -(float)hi.y)};
 }
 
 __device__ __forceinline__ float over_groups_max(float v) {   // over the lanes of a column
@@ -167,21 +173,46 @@ struct Kv4Raw {
     uint4 ks[NB], vs[NB];
 };
 
+// Buffer loads from the group's own resources: their addresses cost no vector instructions.
+template <int W>
+__device__ __forceinline__ void buffer_words(uint32_t (&to)[W], __amdgpu_buffer_rsrc_t r, int at) {
+    static_assert(W == 2 || W == 4 || W == 8, "words of a lane");
+    if constexpr (W == 2) {
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+        to[0] = x.x;
+        to[1] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at + 4 * i, 0, 0));
+            to[i] = x.x;
+            to[i + 1] = x.y;
+            to[i + 2] = x.z;
+            to[i + 3] = x.w;
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t group_buffer(const T* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, bytes, 0x00020000);
+}
+
 template <int NB>
 __device__ __forceinline__ void kv4_load(Kv4Raw<NB>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks,
                                          const uint16_t* vs, int kb, int c, int L) {
-    constexpr int D = 32 * NB;
-    const uint8_t* kp = kc + (size_t)kb * (kv4::kKeys * D / 2) + c * (D / 2) + 4 * L * NB;
-    const uint8_t* vp = vc + (size_t)kb * (kv4::kKeys * D / 2) + (L * 16 + c) * (8 * NB);
+    constexpr int D = 32 * NB, CODES = kv4::kKeys * D / 2;
+    const auto kr = group_buffer(kc + (size_t)kb * CODES, CODES), vr = group_buffer(vc + (size_t)kb * CODES, CODES);
+    const auto sr = group_buffer(ks + (size_t)kb * D, 2 * D), tr = group_buffer(vs + (size_t)kb * D, 2 * D);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) __builtin_memcpy(r.k[u], __builtin_assume_aligned(kp + u * 16 * (D / 2), 4 * NB), 4 * NB);
-    const uint4* kq = reinterpret_cast<const uint4*>(ks + (size_t)kb * D) + L * NB;
-    const uint4* vq = reinterpret_cast<const uint4*>(vs + (size_t)kb * D) + L * NB;
+    for (int u = 0; u < 2; ++u) buffer_words<NB>(r.k[u], kr, (c + 16 * u) * (D / 2) + 4 * L * NB);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) r.ks[b] = kq[b];
-    __builtin_memcpy(r.v, __builtin_assume_aligned(vp, 8 * NB), 8 * NB);
+    for (int b = 0; b < NB; ++b)
+        r.ks[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (L * NB + b), 0, 0));
+    buffer_words<2 * NB>(r.v, vr, (L * 16 + c) * 8 * NB);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) r.vs[b] = vq[b];
+    for (int b = 0; b < NB; ++b)
+        r.vs[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + b), 0, 0));
 }
 
 // Slots 2j and 2j + 1 of a lane's eight scales.
@@ -234,9 +265,11 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
         factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            h2v hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][e] *= up;
-            split8(x[b], qh[n][b], ql[n][b]);
+            for (int e = 0; e < 4; ++e) split2(x[b][2 * e], up, x[b][2 * e + 1], up, hi[e], lo[e]);
+            qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
+            ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
         }
         seen[n] = past + row / a.rep;
         m2[n] = kNegInf;
@@ -247,6 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
 
     // One group of 32 keys.  CAREFUL: some row does not see all of them, or a value
     // block's scale is 2 or more (or no number).
+    const uint32_t magic = magic1024();
     auto group = [&](auto careful, const Kv4Raw<NB>& cur, int key0) {
         constexpr bool CAREFUL = decltype(careful)::value;
         // ---- scores: slots 4u + j of the lane's keys ----
@@ -256,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 h2v k0, k1, k2, k3;
-                codes8(cur.k[u][b], k0, k1, k2, k3);
+                codes8(cur.k[u][b], magic, k0, k1, k2, k3);
                 const h8v ka = h8_of(k0, k1, k2, k3);
                 const h2v d0 = as_h2(word_of(cur.ks[b], 2 * u)), d1 = as_h2(word_of(cur.ks[b], 2 * u + 1));
                 const float dk[4] = {(float)d0.x, (float)d0.y, (float)d1.x, (float)d1.y};
@@ -265,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
                     f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], f4v{}, 0, 0, 0);
                     t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], t, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[n][4 * u + j] = b == 0 ? t[j] * dk[j] : fmaf(t[j], dk[j], s[n][4 * u + j]);
+                    for (int j = 0; j < 4; ++j) s[n][4 * u + j] = fmaf(t[j], dk[j], b == 0 ? 0.f : s[n][4 * u + j]);
                 }
             }
 
@@ -306,8 +340,8 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             h2v v0, v1, v2, v3, w0, w1, w2, w3;
-            codes8(cur.v[2 * b], v0, w0, v1, w1);        // slots 0, 2 and 1, 3: even elements, odd elements
-            codes8(cur.v[2 * b + 1], v2, w2, v3, w3);    // slots 4, 6 and 5, 7
+            codes8(cur.v[2 * b], magic, v0, w0, v1, w1);        // slots 0, 2 and 1, 3: even elements, odd elements
+            codes8(cur.v[2 * b + 1], magic, v2, w2, v3, w3);    // slots 4, 6 and 5, 7
             const h8v va = h8_of(v0, v1, v2, v3), wa = h8_of(w0, w1, w2, w3);
             int down = 0;                                // powers of two that the block's products are formed below
             if constexpr (CAREFUL) {
@@ -322,16 +356,23 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
             const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
-                float x[8];
+                // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.  A key that the row
+                // does not see weighs 0 whatever its scale is.
+                h2v hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const h2v d = as_h2(word_of(cur.vs[b], e >> 1));
-                    const int to = (e & 4) + 2 * (e & 1) + ((e >> 1) & 1);
-                    x[to] = (CAREFUL ? s[n][e] * scale_down : s[n][e]) * (float)((e & 1) ? d.y : d.x);
-                    if constexpr (CAREFUL) x[to] = hidden(n, e) ? 0.f : x[to];   // whatever the scale is
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * (i >> 1) + (i & 1);
+                    const h2v d0 = as_h2(word_of(cur.vs[b], e >> 1)), d1 = as_h2(word_of(cur.vs[b], (e >> 1) + 1));
+                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[n][e], p1 = s[n][e + 2];
+                    if constexpr (CAREFUL) {
+                        f = hidden(n, e) ? 0.f : f;
+                        g = hidden(n, e + 2) ? 0.f : g;
+                        p0 *= scale_down;
+                        p1 *= scale_down;
+                    }
+                    split2(p0, f, p1, g, hi[i], lo[i]);
                 }
-                h8v ph, pl;
-                split8(x, ph, pl);
+                const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
                 if (!CAREFUL || __builtin_amdgcn_readfirstlane(down) == 0) {
                     o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, o[n][2 * b], 0, 0, 0);
                     o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, o[n][2 * b + 1], 0, 0, 0);
