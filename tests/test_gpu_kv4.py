@@ -184,7 +184,7 @@ def test_chunk_attention(ctx, H, G, d, T, n, scale):
 @pytest.mark.parametrize("H,G,d,T,n", [(8, 2, 64, 40, 100), (4, 1, 128, 150, 150), (8, 2, 128, 300, 400), (2, 2, 64, 3, 70)])
 def test_chunk_attention_masked_no_numbers(ctx, H, G, d, T, n):
     """A key or a value that is no number reaches the rows that see it and no other: the others
-    are bit for bit as without it."""
+    are as far from the 64-bit result as they may be without it."""
     print(f"[case] kv4 masked NaN H={H} G={G} d={d} T={T} n={n}", flush=True)
     row = G * d
     K, Vv = (F.normal(88, c, n * row).reshape(n, row) for c in "kv")
@@ -200,8 +200,12 @@ def test_chunk_attention_masked_no_numbers(ctx, H, G, d, T, n):
         kv.attention_chunk(0, q, out, H, T, n, 0.1)
         got[name] = out.download((T, H * d))
     assert np.isfinite(got["none"]).all()
-    assert np.array_equal(got["k"][:1], got["none"][:1]) and np.isnan(got["k"][1:]).all()
-    assert np.array_equal(got["v"][:2], got["none"][:2]) and np.isnan(got["v"][2:]).all()
+    # Groups of keys with such a scale come last, so sums may run in another order: each result
+    # is within the same distance of the exact one.
+    ref, bound = _attention64(q.download((T, H, d)), _decoded(K, n, G, d), _decoded(Vv, n, G, d), H, np.float32(0.1))
+    for name, rows in (("none", T), ("k", 1), ("v", 2)):
+        assert (np.abs(got[name].reshape(ref.shape) - ref) <= bound)[:rows].all(), name
+        assert np.isnan(got[name][rows:]).all(), name
     assert np.isnan(got["first"]).all()
 
 

@@ -618,7 +618,7 @@ static int attn_kv4(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int
         if (rc) return rc;
     }
     return launch_attn_kv4(kv->ctx->stream, q, kv->layers[layer], n_heads, kv->n_kv, kv->d_head, kv->max_seq, T, ctx_len,
-                           scale, out, part);
+                           scale, out, part, kv->ctx->small_tile_ctr);
 }
 
 int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T, int ctx_len,
@@ -671,7 +671,7 @@ int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, fl
     const KVLayer& L = kv->layers[layer];
     if (L.dtype == VLRF_HIP_KV_Q4_0)
         return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out,
-                               kv->ctx->noalloc_scratch);
+                               kv->ctx->noalloc_scratch, kv->ctx->small_tile_ctr);
     return launch_attn_decode(kv->ctx->stream, q, L.k, L.v, L.ks, L.vs, L.dtype, (long)kv->max_seq * kv->d_head,
                               n_heads, kv->n_kv, kv->d_head, ctx_len, nullptr, splits, scale,
                               kv->ctx->noalloc_scratch, out, nullptr, kv->ctx->small_tile_ctr);

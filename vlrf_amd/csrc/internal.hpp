@@ -242,9 +242,9 @@ int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int
                       int T, int pos);
 int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, int ctx_len, float* K,
                        float* V);
-// part: attn_kv4_part_bytes(...) bytes of device memory.
+// part: attn_kv4_part_bytes(...) bytes of device memory; ctr: a context's counters.
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
-                    int ctx_len, float scale, float* out, float* part);
+                    int ctx_len, float scale, float* out, float* part, int* ctr);
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len);
 // Prefill: RoPE on k of T tokens of a [T][ld] QKV buffer at positions
 // pos0.., then the cache append of their K/V rows (q is left as it is: the

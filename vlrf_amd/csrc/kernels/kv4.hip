@@ -9,8 +9,9 @@
 #include "../internal.hpp"
 #include "kv4_layout.hpp"
 
+#include <algorithm>
 #include <cmath>
-#include <type_traits>
+#include <cstdlib>
 
 namespace vlrf_hip {
 namespace {
@@ -103,18 +104,29 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 
 constexpr float kHeadroom = 4.f, kWeightBits = 10.f;
-constexpr int kWaves = 4;
 
 struct Kv4Attn {
     const float* q;          // [T][n_heads][D]
     const uint8_t *kc, *vc;  // the layer's codes and scales
     const uint16_t *ks, *vs;
     float *out, *part;       // [T][n_heads][D]; [T][n_heads][nch][D + 2] where nch > 1
+    int* ctr;                // a counter a block, zero between launches: the merge in this launch; or null
     size_t codes, scales;    // of a head
-    int n_heads, n_kv, rep, T, ctx;
-    int rounds, nch;         // groups of 32 keys a wave takes, chunks of the context
+    int n_heads, rep, T, ctx;
+    uint32_t magic;          // floor(2^32 / rep) + 1: row / rep is the high word of row * magic while row * rep < 2^32
+    int rounds, nch;         // groups of 32 keys a wave takes (tiles: stages a workgroup takes), chunks of the context
     float sl2, qsign;        // |scale| log2(e), the scale's sign
 };
+
+__device__ __forceinline__ int kv4_token(const Kv4Attn& a, int row) {
+    return a.rep == 1 ? row : (int)__umulhi((uint32_t)row, a.magic);
+}
+
+// Row `row` of KV head g among the T * n_heads rows of q.
+__device__ __forceinline__ size_t kv4_q_row(const Kv4Attn& a, int g, int row) {
+    const int t = kv4_token(a, row);
+    return (size_t)t * a.n_heads + g * a.rep + (row - t * a.rep);
+}
 
 __device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
 
@@ -164,13 +176,210 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return t.x + t.y;
 }
 
+// Slots 2j and 2j + 1 of a lane's eight scales.
+__device__ __forceinline__ uint32_t word_of(const uint4& x, int j) { return j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w; }
+
+// The 16 NG rows of a wave: q in two pieces, the factor from a score to powers of two,
+// running maximum and sum, the number of keys that the lane's rows see, O.
+template <int NB, int NG>
+struct Kv4Rows {
+    h8v qh[NG][NB], ql[NG][NB];
+    float factor[NG], m2[NG], l[NG];
+    int seen[NG];
+    f4v o[NG][2 * NB];
+};
+
+template <int NB, int NG>
+__device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn& a, int g, int row0, int R, int c, int L) {
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const int row = min(row0 + 16 * n + c, R - 1);   // rows past the last one repeat it and are not stored
+        const float* qp = a.q + kv4_q_row(a, g, row) * (32 * NB) + 8 * L;
+        float x[NB][8], amax = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float y[8];
+            __builtin_memcpy(y, qp + 32 * b, 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[e];   // in the order of codes8
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
+        }
+        amax = over_groups_max(amax);
+        const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 60);
+        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
+        r.factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            h2v hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split2(x[b][2 * e], up, x[b][2 * e + 1], up, hi[e], lo[e]);
+            r.qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
+            r.ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
+        }
+        r.seen[n] = a.ctx - a.T + 1 + kv4_token(a, row);
+        r.m2[n] = kNegInf;
+        r.l[n] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) r.o[n][t] = f4v{};
+    }
+}
+
+// KG groups of 32 keys from key0 on; src: their operands (k, v) and scales (ks, vs) by
+// group and block.  kEdge: some row does not see all of them; kApart: as well, a value
+// block's scale is 2 or more (or no number).
+enum { kInside, kEdge, kApart };
+
+template <int MODE, int KG, int NB, int NG, class Src>
+__device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int key0, int L) {
+    // ---- scores: slots 4u + j of the lane's keys ----
+    float s[KG][NG][8];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            h8v ka[NB];
+            h2v dk[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) ka[b] = src.k(kg, u, b);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint2 ks = src.ks(kg, u, b);
+                dk[b][0] = as_h2(ks.x);
+                dk[b][1] = as_h2(ks.y);
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                f4v t[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[b], r.ql[n][b], f4v{}, 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[b], r.qh[n][b], t[b], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float& x = s[kg][n][4 * u + j];
+                        x = fmaf(t[b][j], (float)((j & 1) ? dk[b][j >> 1].y : dk[b][j >> 1].x), b == 0 ? 0.f : x);
+                    }
+            }
+        }
+
+    __builtin_amdgcn_sched_barrier(0);   // no loads of the next part early: they would cost registers
+    // ---- softmax ----
+    auto hidden = [&](int kg, int n, int e) { return 32 * kg + kv4::key_of(0, e) >= r.seen[n] - key0 - 4 * L; };
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        float mx = kNegInf;
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (MODE != kInside) s[kg][n][e] = hidden(kg, n, e) ? kNegInf : s[kg][n][e];
+                mx = fmaxf(mx, s[kg][n][e]);
+            }
+        mx = over_groups_max(mx);
+        mx = mx == kNegInf ? kNegInf : mx * r.factor[n];
+        const bool grow = mx > r.m2[n] + kHeadroom;
+        const float mn = grow ? mx : r.m2[n];
+        const float corr = grow ? __builtin_amdgcn_exp2f(r.m2[n] - mn) : 1.f;
+        r.m2[n] = mn;
+        const float at = mn == kNegInf ? 0.f : kWeightBits - mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[kg][n][e] = __builtin_amdgcn_exp2f(fmaf(s[kg][n][e], r.factor[n], at));   // 0 of -inf: the factor is positive
+                sum += s[kg][n][e];
+            }
+        r.l[n] = fmaf(r.l[n], corr, sum);
+        // Without a branch around it, although corr is 1 most of the time: the branch keeps
+        // O in registers twice.
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) r.o[n][t] *= corr;
+    }
+
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- output ----
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            h8v va, wa;   // even elements, odd elements
+            src.v(kg, b, va, wa);
+            const uint4 vs = src.vs(kg, b);
+            int down = 0;                                // powers of two that the block's products are formed below
+            if constexpr (MODE == kApart) {
+                uint32_t top = 15;                       // the largest exponent of the finite scales
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t x = (word_of(vs, j >> 1) >> (16 * (j & 1) + 10)) & 31u;
+                    top = x < 31u ? max(top, x) : top;
+                }
+                down = (int)over_groups_max((float)top) - 15;
+            }
+            const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.  A key that the row
+                // does not see weighs 0 whatever its scale is.
+                h2v hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * (i >> 1) + (i & 1);
+                    const h2v d0 = as_h2(word_of(vs, e >> 1)), d1 = as_h2(word_of(vs, (e >> 1) + 1));
+                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[kg][n][e], p1 = s[kg][n][e + 2];
+                    if constexpr (MODE == kApart) {
+                        f = hidden(kg, n, e) ? 0.f : f;
+                        g = hidden(kg, n, e + 2) ? 0.f : g;
+                        p0 *= scale_down;
+                        p1 *= scale_down;
+                    }
+                    split2(p0, f, p1, g, hi[i], lo[i]);
+                }
+                const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
+                if (MODE != kApart || __builtin_amdgcn_readfirstlane(down) == 0) {
+                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, r.o[n][2 * b], 0, 0, 0);
+                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, r.o[n][2 * b + 1], 0, 0, 0);
+                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, r.o[n][2 * b], 0, 0, 0);
+                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, r.o[n][2 * b + 1], 0, 0, 0);
+                } else {
+                    const float back = __uint_as_float((uint32_t)(127 + down) << 23);
+                    f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, f4v{}, 0, 0, 0);
+                    f4v z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, f4v{}, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, t, 0, 0, 0);
+                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, z, 0, 0, 0);
+                    r.o[n][2 * b] += t * back;
+                    r.o[n][2 * b + 1] += z * back;
+                }
+            }
+        }
+}
+
 // A wave's share of 32 keys as it is loaded: lane (c, L) holds K words of keys c and
 // 16 + c, V bytes of elements 2c, 2c + 1 of each block for the keys of group L, and
 // those keys' scales.
 template <int NB>
 struct Kv4Raw {
-    uint32_t k[2][NB], v[2 * NB];
-    uint4 ks[NB], vs[NB];
+    uint32_t kw[2][NB], vw[2 * NB];
+    uint4 kd[NB], vd[NB];
+    uint32_t magic;
+
+    __device__ __forceinline__ h8v k(int, int u, int b) const {
+        h2v x0, x1, x2, x3;
+        codes8(kw[u][b], magic, x0, x1, x2, x3);
+        return h8_of(x0, x1, x2, x3);
+    }
+    __device__ __forceinline__ void v(int, int b, h8v& even, h8v& odd) const {
+        h2v v0, v1, v2, v3, w0, w1, w2, w3;
+        codes8(vw[2 * b], magic, v0, w0, v1, w1);        // slots (0, 2), (1, 3)
+        codes8(vw[2 * b + 1], magic, v2, w2, v3, w3);    // slots (4, 6), (5, 7)
+        even = h8_of(v0, v1, v2, v3);
+        odd = h8_of(w0, w1, w2, w3);
+    }
+    __device__ __forceinline__ uint2 ks(int, int u, int b) const { return u ? make_uint2(kd[b].z, kd[b].w) : make_uint2(kd[b].x, kd[b].y); }
+    __device__ __forceinline__ uint4 vs(int, int b) const { return vd[b]; }
 };
 
 // Buffer loads from the group's own resources: their addresses cost no vector instructions.
@@ -205,208 +414,140 @@ __device__ __forceinline__ void kv4_load(Kv4Raw<NB>& r, const uint8_t* kc, const
     const auto kr = group_buffer(kc + (size_t)kb * CODES, CODES), vr = group_buffer(vc + (size_t)kb * CODES, CODES);
     const auto sr = group_buffer(ks + (size_t)kb * D, 2 * D), tr = group_buffer(vs + (size_t)kb * D, 2 * D);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) buffer_words<NB>(r.k[u], kr, (c + 16 * u) * (D / 2) + 4 * L * NB);
+    for (int u = 0; u < 2; ++u) buffer_words<NB>(r.kw[u], kr, (c + 16 * u) * (D / 2) + 4 * L * NB);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-        r.ks[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (L * NB + b), 0, 0));
-    buffer_words<2 * NB>(r.v, vr, (L * 16 + c) * 8 * NB);
+        r.kd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (L * NB + b), 0, 0));
+    buffer_words<2 * NB>(r.vw, vr, (L * 16 + c) * 8 * NB);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-        r.vs[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + b), 0, 0));
+        r.vd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + b), 0, 0));
 }
 
-// Slots 2j and 2j + 1 of a lane's eight scales.
-__device__ __forceinline__ uint32_t word_of(const uint4& x, int j) { return j == 0 ? x.x : j == 1 ? x.y : j == 2 ? x.z : x.w; }
+// out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over a row's nch chunks (acc[D],
+// m, l each): wave w of W takes the chunks w, w + W, ..., 16 at a time whose loads
+// are all issued before any is used; the waves merge through LDS (sm, sl, so of the
+// row's waves).  COHERENT: the partials were written by other workgroups of the launch.
+template <int D, int W, bool COHERENT>
+__device__ __forceinline__ void kv4_merge_row(const float* part, int nch, int w, int lane, float* out, float* sm, float* sl,
+                                              float (*so)[D]) {
+    constexpr int B = 16, V = D / 64;
+    float M = kNegInf, sum = 0.f, o[V] = {};
+    const auto pr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, nch * (D + 2) * 4, 0x00020000);
+    auto get = [&](int i) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(pr, 4 * i, 0, COHERENT ? 16 : 0));
+    };
+    for (int c0 = w; c0 < nch; c0 += B * W) {
+        float pm[B], pl[B], po[B][V], mb = M;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int at = min(c0 + b * W, nch - 1) * (D + 2);
+            pm[b] = get(at + D);
+            pl[b] = get(at + D + 1);
+#pragma unroll
+            for (int v = 0; v < V; ++v) po[b][v] = get(at + V * lane + v);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
+        const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+        sum *= f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= f;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const bool on = c0 + b * W < nch && pm[b] != kNegInf;   // an empty chunk has no accumulators
+            const float e = on ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
+            sum += on ? e * pl[b] : 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += on ? e * po[b][v] : 0.f;
+        }
+        M = mb;
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) { sm[w] = M; sl[w] = sum; }
+#pragma unroll
+        for (int v = 0; v < V; ++v) so[w][V * lane + v] = o[v];
+        __syncthreads();
+        if (w) return;
+        const float m0 = M;
+#pragma unroll
+        for (int k = 1; k < W; ++k) M = fmaxf(M, sm[k]);
+        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+        sum *= f0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] *= f0;
+#pragma unroll
+        for (int k = 1; k < W; ++k) {
+            const float f = sm[k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sm[k] - M);
+            sum += f * sl[k];
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] += f * so[k][V * lane + v];
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[V * lane + v] = sum == 0.f ? 0.f : o[v] / sum;
+}
+
+// Waves of a workgroup of NG groups of 16 rows.
+constexpr int kv4_waves(int groups) { return groups == 1 ? 8 : 4; }
 
 template <int D, int NG>
-__global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_kernel(Kv4Attn a) {
-    constexpr int NB = D / 32, ROWS = 16 * NG, OS = D + 4;
+__global__ __launch_bounds__(64 * kv4_waves(NG), NG == 1 ? 2 : 1) void kv4_attn_rows_kernel(Kv4Attn a) {
+    constexpr int NB = D / 32, ROWS = 16 * NG, OS = D + 4, kWaves = kv4_waves(NG);
+    __shared__ int last;
     __shared__ __align__(16) float os[kWaves][ROWS * OS];
     __shared__ float ms[kWaves][ROWS], ls[kWaves][ROWS];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
-    const int nch = a.nch, chunk = blockIdx.x % nch, blk = blockIdx.x / nch;
-    const int g = blk % a.n_kv, row0 = blk / a.n_kv * ROWS, R = a.T * a.rep;
+    const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, row0 = blockIdx.z * ROWS, R = a.T * a.rep;
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
     const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
-    auto q_row = [&](int row) {   // of the T * n_heads rows of q
-        const int t = row / a.rep;
-        return (size_t)t * a.n_heads + g * a.rep + (row - t * a.rep);
-    };
-    // Keys that the block's first and last row see; the lane's rows' own.
-    const int past = a.ctx - a.T + 1;
-    const int fewest = past + row0 / a.rep, most = past + min(row0 + ROWS - 1, R - 1) / a.rep;
+    // Keys that the block's first and last row see.
+    const int past = a.ctx - a.T + 1, fewest = past + kv4_token(a, row0), most = past + kv4_token(a, min(row0 + ROWS - 1, R - 1));
     const int kb0 = chunk * kWaves * a.rounds + w;
     const int mine = min(a.rounds, max(0, ((most + kv4::kKeys - 1) / kv4::kKeys - kb0 + kWaves - 1) / kWaves));
 
     Kv4Raw<NB> raw;
+    raw.magic = magic1024();
     if (mine > 0) kv4_load<NB>(raw, kc, vc, ks, vs, kb0, c, L);
-
-    h8v qh[NG][NB], ql[NG][NB];
-    float factor[NG], m2[NG], l[NG];
-    int seen[NG];
-    f4v o[NG][2 * NB];
+    Kv4Rows<NB, NG> r;
+    kv4_rows_init<NB, NG>(r, a, g, row0, R, c, L);
+    // Three loops of one body each (two in one would cost each other registers): the groups
+    // that every row sees whole, those at some row's edge, and those of both that the first
+    // two left because of a large scale.
+    const int inside = max(0, min(mine, (fewest / kv4::kKeys - kb0 + kWaves - 1) / kWaves));
+    bool left = false;
+    auto large = [&](const Kv4Raw<NB>& x) {   // a scale of 2 or more, or no number
+        uint32_t any = 0;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-        const int row = min(row0 + 16 * n + c, R - 1);
-        const float* qp = a.q + q_row(row) * D + 8 * L;
-        float x[NB][8], amax = 0.f;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float y[8];
-            __builtin_memcpy(y, qp + 32 * b, 32);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[e];   // in the order of codes8
-#pragma unroll
-            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
-        }
-        amax = over_groups_max(amax);
-        const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 120);
-        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-        factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            h2v hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(x[b][2 * e], up, x[b][2 * e + 1], up, hi[e], lo[e]);
-            qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
-            ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
-        }
-        seen[n] = past + row / a.rep;
-        m2[n] = kNegInf;
-        l[n] = 0.f;
-#pragma unroll
-        for (int t = 0; t < 2 * NB; ++t) o[n][t] = f4v{};
-    }
-
-    // One group of 32 keys.  CAREFUL: some row does not see all of them, or a value
-    // block's scale is 2 or more (or no number).
-    const uint32_t magic = magic1024();
-    auto group = [&](auto careful, const Kv4Raw<NB>& cur, int key0) {
-        constexpr bool CAREFUL = decltype(careful)::value;
-        // ---- scores: slots 4u + j of the lane's keys ----
-        float s[NG][8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                h2v k0, k1, k2, k3;
-                codes8(cur.k[u][b], magic, k0, k1, k2, k3);
-                const h8v ka = h8_of(k0, k1, k2, k3);
-                const h2v d0 = as_h2(word_of(cur.ks[b], 2 * u)), d1 = as_h2(word_of(cur.ks[b], 2 * u + 1));
-                const float dk[4] = {(float)d0.x, (float)d0.y, (float)d1.x, (float)d1.y};
-#pragma unroll
-                for (int n = 0; n < NG; ++n) {
-                    f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[n][b], f4v{}, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[n][b], t, 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[n][4 * u + j] = fmaf(t[j], dk[j], b == 0 ? 0.f : s[n][4 * u + j]);
-                }
-            }
-
-        // ---- softmax ----
-        auto hidden = [&](int n, int e) { return key0 + kv4::key_of(L, e) >= seen[n]; };
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (CAREFUL) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[n][e] = hidden(n, e) ? kNegInf : s[n][e];
-            }
-            float mx = s[n][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[n][e]);
-            mx = over_groups_max(mx);
-            mx = mx == kNegInf ? kNegInf : mx * factor[n];
-            const bool grow = mx > m2[n] + kHeadroom;
-            const float mn = grow ? mx : m2[n];
-            const float corr = grow ? __builtin_amdgcn_exp2f(m2[n] - mn) : 1.f;
-            m2[n] = mn;
-            const float at = mn == kNegInf ? 0.f : kWeightBits - mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float p = __builtin_amdgcn_exp2f(fmaf(s[n][e], factor[n], at));
-                if constexpr (CAREFUL) p = hidden(n, e) ? 0.f : p;
-                s[n][e] = p;
-                sum += p;
-            }
-            l[n] = fmaf(l[n], corr, sum);
-            if (__builtin_amdgcn_ballot_w64(grow)) {
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) o[n][t] *= corr;
-            }
-        }
-
-        // ---- output ----
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            h2v v0, v1, v2, v3, w0, w1, w2, w3;
-            codes8(cur.v[2 * b], magic, v0, w0, v1, w1);        // slots 0, 2 and 1, 3: even elements, odd elements
-            codes8(cur.v[2 * b + 1], magic, v2, w2, v3, w3);    // slots 4, 6 and 5, 7
-            const h8v va = h8_of(v0, v1, v2, v3), wa = h8_of(w0, w1, w2, w3);
-            int down = 0;                                // powers of two that the block's products are formed below
-            if constexpr (CAREFUL) {
-                uint32_t top = 15;                       // the largest exponent of the finite scales
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t x = (word_of(cur.vs[b], j >> 1) >> (16 * (j & 1) + 10)) & 31u;
-                    top = x < 31u ? max(top, x) : top;
-                }
-                down = (int)over_groups_max((float)top) - 15;
-            }
-            const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.  A key that the row
-                // does not see weighs 0 whatever its scale is.
-                h2v hi[4], lo[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 4 * (i >> 1) + (i & 1);
-                    const h2v d0 = as_h2(word_of(cur.vs[b], e >> 1)), d1 = as_h2(word_of(cur.vs[b], (e >> 1) + 1));
-                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[n][e], p1 = s[n][e + 2];
-                    if constexpr (CAREFUL) {
-                        f = hidden(n, e) ? 0.f : f;
-                        g = hidden(n, e + 2) ? 0.f : g;
-                        p0 *= scale_down;
-                        p1 *= scale_down;
-                    }
-                    split2(p0, f, p1, g, hi[i], lo[i]);
-                }
-                const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
-                if (!CAREFUL || __builtin_amdgcn_readfirstlane(down) == 0) {
-                    o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, o[n][2 * b], 0, 0, 0);
-                    o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, o[n][2 * b + 1], 0, 0, 0);
-                    o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, o[n][2 * b], 0, 0, 0);
-                    o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, o[n][2 * b + 1], 0, 0, 0);
-                } else {
-                    const float back = __uint_as_float((uint32_t)(127 + down) << 23);
-                    f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, f4v{}, 0, 0, 0);
-                    f4v z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, f4v{}, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, t, 0, 0, 0);
-                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, z, 0, 0, 0);
-                    o[n][2 * b] += t * back;
-                    o[n][2 * b + 1] += z * back;
-                }
-            }
-        }
+        for (int b = 0; b < NB; ++b) any |= x.vd[b].x | x.vd[b].y | x.vd[b].z | x.vd[b].w;
+        return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
     };
-    for (int i = 0; i < mine; ++i) {
-        const int kb = kb0 + i * kWaves, key0 = kb * kv4::kKeys;
+    auto load = [&](int i) { kv4_load<NB>(raw, kc, vc, ks, vs, kb0 + i * kWaves, c, L); };   // i < mine
+    int i = 0;
+    for (; i < inside; ++i) {
         const Kv4Raw<NB> cur = raw;
-        if (i + 1 < mine) kv4_load<NB>(raw, kc, vc, ks, vs, kb + kWaves, c, L);
-        uint32_t large = 0;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) large |= cur.vs[b].x | cur.vs[b].y | cur.vs[b].z | cur.vs[b].w;
-        if (key0 + kv4::kKeys > fewest || __builtin_amdgcn_ballot_w64((large & 0x40004000u) != 0)) group(std::true_type(), cur, key0);
-        else group(std::false_type(), cur, key0);
+        if (i + 1 < mine) load(i + 1);
+        if (large(cur)) left = true;
+        else kv4_keys<kInside, 1>(r, cur, (kb0 + i * kWaves) * kv4::kKeys, L);
     }
+    for (; i < mine; ++i) {
+        const Kv4Raw<NB> cur = raw;
+        if (i + 1 < mine) load(i + 1);
+        if (large(cur)) left = true;
+        else kv4_keys<kEdge, 1>(r, cur, (kb0 + i * kWaves) * kv4::kKeys, L);
+    }
+    if (left)
+        for (i = 0; i < mine; ++i) {
+            load(i);
+            if (large(raw)) kv4_keys<kApart, 1>(r, raw, (kb0 + i * kWaves) * kv4::kKeys, L);
+        }
 
     // ---- the waves' results, then the chunk's ----
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-        const float sum = over_groups_sum(l[n]);
+        const float sum = over_groups_sum(r.l[n]);
         if (L == 0) {
-            ms[w][16 * n + c] = sum != sum ? INFINITY : m2[n];   // a NaN has to win where the others' weights would drop it
+            ms[w][16 * n + c] = sum != sum ? INFINITY : r.m2[n];   // a NaN has to win where the others' weights would drop it
             ls[w][16 * n + c] = sum;
         }
 #pragma unroll
@@ -414,26 +555,34 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 *reinterpret_cast<float4*>(&os[w][(16 * n + c) * OS + 32 * b + 8 * L + 4 * h]) =
-                    make_float4(o[n][2 * b][2 * h], o[n][2 * b + 1][2 * h], o[n][2 * b][2 * h + 1], o[n][2 * b + 1][2 * h + 1]);
+                    make_float4(r.o[n][2 * b][2 * h], r.o[n][2 * b + 1][2 * h], r.o[n][2 * b][2 * h + 1], r.o[n][2 * b + 1][2 * h + 1]);
     }
     __syncthreads();
     const int rows = min(ROWS, R - row0);
     for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) {
-        const int r = i / D, e = i - r * D;
-        float M = ms[0][r], sum = 0.f, x = 0.f;
+        const int k0 = i / D, e = i - k0 * D;
+        float M = ms[0][k0], sum = 0.f, x = 0.f;
 #pragma unroll
-        for (int k = 1; k < kWaves; ++k) M = fmaxf(M, ms[k][r]);
+        for (int k = 1; k < kWaves; ++k) M = fmaxf(M, ms[k][k0]);
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            const float f = ms[k][r] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms[k][r] - M);
-            sum += f * ls[k][r];
-            x += f * os[k][r * OS + e];
+            const float f = ms[k][k0] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms[k][k0] - M);
+            sum += f * ls[k][k0];
+            x += f * os[k][k0 * OS + e];
         }
-        const size_t at = q_row(row0 + r);
+        const size_t at = kv4_q_row(a, g, row0 + k0);
         if (nch == 1) {
             a.out[at * D + e] = sum == 0.f ? 0.f : x / sum;
+            continue;
+        }
+        float* p = a.part + (at * nch + chunk) * (D + 2);
+        if (a.ctr) {   // read by another workgroup of this launch
+            __hip_atomic_store(p + e, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (e == 0) {
+                __hip_atomic_store(p + D, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(p + D + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         } else {
-            float* p = a.part + (at * nch + chunk) * (D + 2);
             p[e] = x;
             if (e == 0) {
                 p[D] = M;
@@ -441,71 +590,201 @@ __global__ __launch_bounds__(64 * kWaves, NG == 1 ? 2 : 1) void kv4_attn_rows_ke
             }
         }
     }
+    if (nch == 1 || !a.ctr) return;
+
+    // ---- the workgroup that comes last merges the block's chunks, in their order ----
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's stores acknowledged (vmcnt 0)
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* ctr = a.ctr + (size_t)(blockIdx.z * gridDim.y + g) * kSmallTileCtrStride;
+        last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nch - 1;
+        if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int i = w; i < rows; i += kWaves) {
+        const size_t at = kv4_q_row(a, g, row0 + i);
+        kv4_merge_row<D, 1, true>(a.part + at * nch * (D + 2), nch, 0, lane, a.out + at * D, nullptr, nullptr, nullptr);
+    }
 }
 
-// out[row] = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the row's chunks.  W
-// waves a row (eight a workgroup), wave w's chunks w, w + W, ..., eight at a time
-// whose loads are all issued before any is used; the waves merge through LDS.
+// ---- many rows --------------------------------------------------------------------
+// Four waves of 32 rows share what they read: a stage of 8192 / D keys is decoded once,
+// into LDS, where the operands stand as the lanes read them (a wave decodes a quarter of
+// the stage's K and of its V).  Stages alternate between two buffers, one barrier a
+// stage; the next one's codes are in registers meanwhile.  Each wave keeps its rows to
+// the end, so nothing is merged but chunks of keys where there are few rows.  Three
+// passes over the stages, as above.
+constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
+
+template <int NB>
+struct Kv4Stage {
+    static constexpr int GROUPS = 8 / NB, KEYS = 32 * GROUPS;
+    uint4 k[16][64], v[16][64];    // [group][2 NB][lane]
+    uint4 kd[32], vd[32];          // [group][L][block]
+    uint32_t large[2];             // a scale of 2 or more among a half of vd
+};
+
+template <int NB>
+struct Kv4FromStage {
+    const Kv4Stage<NB>& st;
+    int group, lane;
+    __device__ __forceinline__ h8v k(int kg, int u, int b) const {
+        return __builtin_bit_cast(h8v, st.k[(2 * (group + kg) + u) * NB + b][lane]);
+    }
+    __device__ __forceinline__ void v(int kg, int b, h8v& even, h8v& odd) const {
+        even = __builtin_bit_cast(h8v, st.v[2 * ((group + kg) * NB + b)][lane]);
+        odd = __builtin_bit_cast(h8v, st.v[2 * ((group + kg) * NB + b) + 1][lane]);
+    }
+    __device__ __forceinline__ uint2 ks(int kg, int u, int b) const {
+        return reinterpret_cast<const uint2*>(&st.kd[(4 * (group + kg) + (lane >> 4)) * NB + b])[u];
+    }
+    __device__ __forceinline__ uint4 vs(int kg, int b) const { return st.vd[(4 * (group + kg) + (lane >> 4)) * NB + b]; }
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4Attn a) {
+    constexpr int NB = D / 32, NG = 2, ROWS = 16 * NG;
+    using Stage = Kv4Stage<NB>;
+    constexpr int PAIRS = Stage::GROUPS / 2;
+    __shared__ Stage stage[2];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
+    const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, R = a.T * a.rep, past = a.ctx - a.T + 1;
+    // The first workgroups, one a CU, take the longest rows from the last block down; the
+    // others the shortest ones up.
+    const int nblk = gridDim.z, ahead = min(nblk, (256 + nch * (int)gridDim.y - 1) / (nch * (int)gridDim.y)), z = blockIdx.z;
+    const int block = z < ahead ? nblk - 1 - z : z - ahead;
+    const int row0 = block * kTileRows + ROWS * w;
+    auto keys_of = [&](int row) { return past + kv4_token(a, min(row, R - 1)); };
+    const int most = row0 < R ? keys_of(row0 + ROWS - 1) : 0;
+    const int s0 = chunk * a.rounds;
+    const int s1 = min(s0 + a.rounds, (keys_of(block * kTileRows + kTileRows - 1) + Stage::KEYS - 1) / Stage::KEYS);
+    const int inside = min(s1, keys_of(block * kTileRows) / Stage::KEYS);   // stages below it are whole for every row
+
+    // This wave's runs of a stage: 1 KiB of K, of V, and (lanes 0..15) half of the scales of K (waves 0, 1) or V.
+    const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
+    const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
+    const uint32_t magic = magic1024();
+    uint32_t kw[4], vw[4];
+    uint4 sc;
+    auto fetch = [&](int s) {   // past the cache's end: zeros
+        const size_t at = (size_t)s * 4096, sat = (size_t)s * 256;   // bytes of codes, f16 scales
+        const int left = (int)min((size_t)4096, a.codes - at), sleft = (int)min((size_t)256, a.scales - sat) * 2;
+        const auto kr = group_buffer(kc + at, left), vr = group_buffer(vc + at, left);
+        if constexpr (D == 64) {   // a run of K holds both halves of a group's keys, 8 bytes a lane
+            uint32_t x[2], y[2];
+            buffer_words<2>(x, kr, 1024 * w + c * 32 + 8 * L);
+            buffer_words<2>(y, kr, 1024 * w + (c + 16) * 32 + 8 * L);
+            kw[0] = x[0]; kw[1] = x[1]; kw[2] = y[0]; kw[3] = y[1];
+            buffer_words<4>(vw, vr, 1024 * w + (L * 16 + c) * 16);
+        } else {
+            buffer_words<4>(kw, kr, 1024 * w + c * 64 + 16 * L);
+            buffer_words<4>(vw, vr, 2048 * (w >> 1) + (L * 16 + c) * 32 + 16 * (w & 1));
+        }
+        const auto sr = group_buffer((w & 2) ? vs + sat : ks + sat, sleft);
+        sc = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (16 * (w & 1) + c), 0, 0));
+    };
+    auto put = [&](Stage& st) {
+        h2v x0, x1, x2, x3, y0, y1, y2, y3;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            codes8(kw[j], magic, x0, x1, x2, x3);
+            st.k[4 * w + j][lane] = __builtin_bit_cast(uint4, h8_of(x0, x1, x2, x3));
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            codes8(vw[2 * j], magic, x0, x1, x2, x3);
+            codes8(vw[2 * j + 1], magic, y0, y1, y2, y3);
+            st.v[4 * w + 2 * j][lane] = __builtin_bit_cast(uint4, h8_of(x0, x2, y0, y2));
+            st.v[4 * w + 2 * j + 1][lane] = __builtin_bit_cast(uint4, h8_of(x1, x3, y1, y3));
+        }
+        if (lane < 16) ((w & 2) ? st.vd : st.kd)[16 * (w & 1) + lane] = sc;
+        const bool big = __builtin_amdgcn_ballot_w64(((sc.x | sc.y | sc.z | sc.w) & 0x40004000u) != 0) != 0;
+        if (lane == 0 && (w & 2)) st.large[w & 1] = big;
+    };
+    // The stages [from, to): body(stage, s) with each one in LDS.
+    auto stages = [&](int from, int to, auto body) {
+        if (from >= to) return;
+        fetch(from);
+        put(stage[0]);
+        if (from + 1 < to) fetch(from + 1);
+        __syncthreads();
+        for (int s = from; s < to; ++s) {
+            body(stage[(s - from) & 1], s);
+            if (s + 1 < to) {   // into the buffer of stage s - 1: every wave is past its barrier
+                put(stage[(s + 1 - from) & 1]);
+                if (s + 2 < to) fetch(s + 2);
+            }
+            __syncthreads();
+        }
+    };
+    auto is_large = [&](const Stage& st) {
+        return __builtin_amdgcn_readfirstlane(st.large[0] | st.large[1]) != 0;
+    };
+
+    Kv4Rows<NB, NG> r;
+    kv4_rows_init<NB, NG>(r, a, g, min(row0, R - 1), R, c, L);
+    bool left = false;
+    stages(s0, inside, [&](const Stage& st, int s) {
+        if (is_large(st)) {
+            left = true;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i)
+            kv4_keys<kInside, 2>(r, Kv4FromStage<NB>{st, 2 * i, lane}, s * Stage::KEYS + 64 * i, L);
+    });
+    stages(max(s0, inside), s1, [&](const Stage& st, int s) {
+        if (is_large(st)) {
+            left = true;
+            return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < PAIRS; ++i) {
+            const int key0 = s * Stage::KEYS + 64 * i;
+            if (key0 < most) kv4_keys<kEdge, 2>(r, Kv4FromStage<NB>{st, 2 * i, lane}, key0, L);
+        }
+    });
+    if (left)
+        stages(s0, s1, [&](const Stage& st, int s) {
+            if (!is_large(st)) return;
+#pragma unroll 1
+            for (int i = 0; i < Stage::GROUPS; ++i) {
+                const int key0 = s * Stage::KEYS + 32 * i;
+                if (key0 < most) kv4_keys<kApart, 1>(r, Kv4FromStage<NB>{st, i, lane}, key0, L);
+            }
+        });
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const float sum = over_groups_sum(r.l[n]);
+        const int row = row0 + 16 * n + c;
+        if (row >= R) continue;
+        const size_t at = kv4_q_row(a, g, row);
+        float* to = nch == 1 ? a.out + at * D : a.part + (at * nch + chunk) * (D + 2);
+        const float by = nch > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float x[4] = {r.o[n][2 * b][2 * h] * by, r.o[n][2 * b + 1][2 * h] * by, r.o[n][2 * b][2 * h + 1] * by,
+                                    r.o[n][2 * b + 1][2 * h + 1] * by};
+                __builtin_memcpy(to + 32 * b + 8 * L + 4 * h, x, 16);
+            }
+        if (nch > 1 && L == 0) {
+            to[D] = sum != sum ? INFINITY : r.m2[n];
+            to[D + 1] = sum;
+        }
+    }
+}
+
+// The merge as a launch of its own: W waves a row, eight a workgroup.
 template <int D, int W>
 __global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, int rows,
                                                         float* __restrict__ out) {
-    constexpr int B = 8, V = D / 64;
     __shared__ float sm[8], sl[8], so[8][D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
-    const int row = (int)blockIdx.x * (8 / W) + wave / W;
-    float M = kNegInf, sum = 0.f, o[V] = {};
-    if (row < rows) {
-        const float* p = part + (size_t)row * nch * (D + 2);
-        for (int c0 = w; c0 < nch; c0 += B * W) {
-            float pm[B], pl[B], po[B][V], mb = M;
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const float* pc = p + (size_t)min(c0 + b * W, nch - 1) * (D + 2);
-                pm[b] = pc[D];
-                pl[b] = pc[D + 1];
-                __builtin_memcpy(po[b], __builtin_assume_aligned(pc + V * lane, 4 * V), 4 * V);
-            }
-#pragma unroll
-            for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
-            const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
-            sum *= f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] *= f;
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const bool on = c0 + b * W < nch && pm[b] != kNegInf;   // an empty chunk has no accumulators
-                const float e = on ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
-                sum += on ? e * pl[b] : 0.f;
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[v] += on ? e * po[b][v] : 0.f;
-            }
-            M = mb;
-        }
-    }
-    if constexpr (W > 1) {
-        if (lane == 0) { sm[wave] = M; sl[wave] = sum; }
-#pragma unroll
-        for (int v = 0; v < V; ++v) so[wave][V * lane + v] = o[v];
-        __syncthreads();
-        if (w) return;
-        const float m0 = M;
-#pragma unroll
-        for (int k = 1; k < W; ++k) M = fmaxf(M, sm[wave + k]);
-        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
-        sum *= f0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] *= f0;
-#pragma unroll
-        for (int k = 1; k < W; ++k) {
-            const float f = sm[wave + k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sm[wave + k] - M);
-            sum += f * sl[wave + k];
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] += f * so[wave + k][V * lane + v];
-        }
-    }
-    if (row >= rows) return;
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[(size_t)row * D + V * lane + v] = sum == 0.f ? 0.f : o[v] / sum;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = (int)blockIdx.x * (8 / W) + wave / W;
+    if (W == 1 && row >= rows) return;   // W 8: a row a workgroup
+    kv4_merge_row<D, W, false>(part + (size_t)row * nch * (D + 2), nch, wave % W, lane, out + (size_t)row * D, sm, sl, so);
 }
 
 }  // namespace
@@ -535,39 +814,53 @@ int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, in
 }
 
 namespace {
-// Workgroups of a launch: ROWS rows a block, `rounds` groups of 32 keys a wave.
 struct Kv4Plan {
-    int groups = 1, blocks = 1, rounds = 1, nch = 1;   // 16-row groups a block, blocks (KV heads included)
+    int groups = 1;                          // 16-row groups a block of the rows kernel; 0: the tiles kernel
+    int blocks = 1, rounds = 1, nch = 1;     // blocks of rows of a KV head
 };
 
-Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
+Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
     const long R = (long)T * (n_heads / n_kv);
+    const char* e = std::getenv("KV4_TILES");
+    const long from = e ? atol(e) : 64;
+    if (R >= from) {
+        const long nb = (ctx_len + 8192 / d_head - 1) / (8192 / d_head), want = 512;   // stages, workgroups
+        p.groups = 0;
+        p.blocks = (int)((R + kTileRows - 1) / kTileRows);
+        long nch = std::max(1l, want / ((long)p.blocks * n_kv));
+        nch = std::min(nch, nb);
+        p.rounds = (int)((nb + nch - 1) / nch);
+        p.nch = (int)((nb + p.rounds - 1) / p.rounds);
+        return p;
+    }
     p.groups = R > 16 ? 2 : 1;
-    p.blocks = (int)((R + 16 * p.groups - 1) / (16 * p.groups)) * n_kv;
+    if (const char* f = std::getenv("KV4_G")) p.groups = atoi(f);
+    p.blocks = (int)((R + 16 * p.groups - 1) / (16 * p.groups));
     const long nb = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
-    const long want = 512;
-    p.rounds = (int)((nb * p.blocks + kWaves * want - 1) / (kWaves * want));
-    p.nch = (int)((nb + kWaves * p.rounds - 1) / (kWaves * p.rounds));
+    const long waves = kv4_waves(p.groups), want = 2048 / waves;
+    p.rounds = (int)((nb * p.blocks * n_kv + waves * want - 1) / (waves * want));
+    p.nch = (int)((nb + waves * p.rounds - 1) / (waves * p.rounds));
     return p;
 }
 }  // namespace
 
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1) return 0;   // refused by the launch
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
     return p.nch > 1 ? (size_t)T * n_heads * p.nch * (d_head + 2) * sizeof(float) : 0;
 }
 
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
-                    int ctx_len, float scale, float* out, float* part) {
+                    int ctx_len, float scale, float* out, float* part, int* ctr) {
     VH_ARG(n_kv >= 1 && n_heads >= 1 && n_heads % n_kv == 0, "attn: n_heads %d not a multiple of n_kv %d", n_heads, n_kv);
     VH_ARG(d_head == 64 || d_head == 128, "attn: d_head %d not in {64,128}", d_head);
     VH_ARG(ctx_len >= 1 && ctx_len <= max_seq && T >= 1 && T <= ctx_len, "attn: %d rows of %d keys in a cache of %d", T,
            ctx_len, max_seq);
     VH_ARG((long)T * n_heads < (1l << 31), "attn: %d rows of %d heads", T, n_heads);
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
-    VH_ARG((long)p.blocks * p.nch < (1l << 31), "attn: %d rows of %d heads over %d keys", T, n_heads, ctx_len);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
+    VH_ARG(p.blocks <= 65535 && n_kv <= 65535 && (size_t)T * n_heads / n_kv * (n_heads / n_kv) < (1ull << 32),
+           "attn: %d rows of %d heads over %d KV heads are beyond a launch", T, n_heads, n_kv);
     VH_ARG(p.nch == 1 || part, "attn: no scratch");
     Kv4Attn a;
     a.q = q;
@@ -577,20 +870,26 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     a.vs = reinterpret_cast<const uint16_t*>(L.vs);
     a.out = out;
     a.part = part;
+    const bool merged = ctr && p.groups == 1 && (long)p.blocks * n_kv <= kSmallMaxTiles && p.nch <= 32;
+    a.ctr = merged ? ctr : nullptr;
     a.codes = kv4::head_codes(max_seq, d_head);
     a.scales = kv4::head_scales(max_seq, d_head);
     a.n_heads = n_heads;
-    a.n_kv = n_kv;
     a.rep = n_heads / n_kv;
+    a.magic = (uint32_t)((1ull << 32) / a.rep + 1);
     a.T = T;
     a.ctx = ctx_len;
     a.rounds = p.rounds;
     a.nch = p.nch;
-    a.sl2 = (float)(std::fabs((double)scale) * 1.4426950408889634);
+    // Never 0: a masked score's -inf times the factor has to stay -inf.
+    a.sl2 = std::max((float)(std::fabs((double)scale) * 1.4426950408889634), 1e-20f);
     a.qsign = scale < 0.f ? -1.f : 1.f;
-    const dim3 grid((unsigned)((long)p.blocks * p.nch));
-#define VH_ROWS(D, G) VH_LAUNCH((kv4_attn_rows_kernel<D, G>), grid, dim3(64 * kWaves), 0, s, a)
-    if (d_head == 64) {
+    const dim3 grid(p.nch, n_kv, p.blocks);
+#define VH_ROWS(D, G) VH_LAUNCH((kv4_attn_rows_kernel<D, G>), grid, dim3(64 * kv4_waves(G)), 0, s, a)
+    if (p.groups == 0) {
+        if (d_head == 64) VH_LAUNCH(kv4_attn_tiles_kernel<64>, grid, dim3(64 * kTileWaves), 0, s, a);
+        else VH_LAUNCH(kv4_attn_tiles_kernel<128>, grid, dim3(64 * kTileWaves), 0, s, a);
+    } else if (d_head == 64) {
         if (p.groups == 1) VH_ROWS(64, 1);
         else VH_ROWS(64, 2);
     } else {
@@ -599,7 +898,7 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     }
 #undef VH_ROWS
     VH_LAUNCHED();
-    if (p.nch == 1) return VLRF_HIP_OK;
+    if (p.nch == 1 || merged) return VLRF_HIP_OK;
     const int rows = T * n_heads;
 #define VH_MERGE(D, W) \
     VH_LAUNCH((kv4_merge_kernel<D, W>), dim3((rows + 8 / W - 1) / (8 / W)), dim3(512), 0, s, part, p.nch, rows, out)
