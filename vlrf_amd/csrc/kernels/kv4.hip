@@ -114,7 +114,7 @@ struct Kv4Attn {
     size_t codes, scales;    // of a head
     int n_heads, rep, T, ctx;
     uint32_t magic;          // floor(2^32 / rep) + 1: row / rep is the high word of row * magic while row * rep < 2^32
-    int rounds, nch;         // groups of 32 keys a wave takes (tiles: stages a workgroup takes), chunks of the context
+    int rounds, nch;         // groups of 32 keys a wave takes, chunks of the context
     float sl2, qsign;        // |scale| log2(e), the scale's sign
 };
 
@@ -424,79 +424,102 @@ __device__ __forceinline__ void kv4_load(Kv4Raw<NB>& r, const uint8_t* kc, const
         r.vd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + b), 0, 0));
 }
 
-// out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over a row's nch chunks (acc[D],
-// m, l each): wave w of W takes the chunks w, w + W, ..., 16 at a time whose loads
-// are all issued before any is used; the waves merge through LDS (sm, sl, so of the
-// row's waves).  COHERENT: the partials were written by other workgroups of the launch.
-template <int D, int W, bool COHERENT>
-__device__ __forceinline__ void kv4_merge_row(const float* part, int nch, int w, int lane, float* out, float* sm, float* sl,
-                                              float (*so)[D]) {
-    constexpr int B = 16, V = D / 64;
-    float M = kNegInf, sum = 0.f, o[V] = {};
-    const auto pr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, nch * (D + 2) * 4, 0x00020000);
-    auto get = [&](int i) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(pr, 4 * i, 0, COHERENT ? 16 : 0));
-    };
-    for (int c0 = w; c0 < nch; c0 += B * W) {
-        float pm[B], pl[B], po[B][V], mb = M;
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int at = min(c0 + b * W, nch - 1) * (D + 2);
-            pm[b] = get(at + D);
-            pl[b] = get(at + D + 1);
-#pragma unroll
-            for (int v = 0; v < V; ++v) po[b][v] = get(at + V * lane + v);
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
-        const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
-        sum *= f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] *= f;
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const bool on = c0 + b * W < nch && pm[b] != kNegInf;   // an empty chunk has no accumulators
-            const float e = on ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
-            sum += on ? e * pl[b] : 0.f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] += on ? e * po[b][v] : 0.f;
-        }
-        M = mb;
-    }
-    if constexpr (W > 1) {
-        if (lane == 0) { sm[w] = M; sl[w] = sum; }
-#pragma unroll
-        for (int v = 0; v < V; ++v) so[w][V * lane + v] = o[v];
-        __syncthreads();
-        if (w) return;
-        const float m0 = M;
-#pragma unroll
-        for (int k = 1; k < W; ++k) M = fmaxf(M, sm[k]);
-        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
-        sum *= f0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] *= f0;
-#pragma unroll
-        for (int k = 1; k < W; ++k) {
-            const float f = sm[k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sm[k] - M);
-            sum += f * sl[k];
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] += f * so[k][V * lane + v];
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[V * lane + v] = sum == 0.f ? 0.f : o[v] / sum;
+// A chunk's partial of a row: acc[D], m, l and two floats that align the next.  The host
+// keeps all of a launch below 2 GiB.
+constexpr int kv4_part(int d) { return d + 4; }
+typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+typedef unsigned int u2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(const float* part) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, 0x7fffffff, 0x00020000);
 }
 
-// Waves of a workgroup of NG groups of 16 rows.
-constexpr int kv4_waves(int groups) { return groups == 1 ? 8 : 4; }
+// out[row] = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the nch chunks of `rows`
+// rows, by a workgroup of 512.  A thread takes four elements of a row, and where rows
+// are few several threads share the chunks: c, c + P, ..., eight at a time whose loads
+// are all issued before any is used; they merge through LDS.  row_at: the row's place.
+// COHERENT: the partials were written by other workgroups of the launch.
+template <int D>
+struct Kv4MergeLds {
+    float4 o[512];
+    float m[512], l[512];
+};
 
-template <int D, int NG>
-__global__ __launch_bounds__(64 * kv4_waves(NG), NG == 1 ? 2 : 1) void kv4_attn_rows_kernel(Kv4Attn a) {
-    constexpr int NB = D / 32, ROWS = 16 * NG, OS = D + 4, kWaves = kv4_waves(NG);
+template <int D, bool COHERENT, class At>
+__device__ __forceinline__ void kv4_merge(Kv4MergeLds<D>& sm, const float* part, int nch, int rows, float* out, At row_at) {
+    constexpr int B = 8, Q = D / 4, PS = kv4_part(D), AUX = COHERENT ? 16 : 0;   // 16: sc1, past this die's L2
+    const int n = rows * Q, P = 512 / n, tid = threadIdx.x, share = tid / n, i = tid - share * n;
+    const bool on = share < P;
+    const size_t at = row_at(on ? i / Q : 0);
+    const auto pr = part_buffer(part);
+    const int first = (int)(4 * at * nch * PS);
+    float M = kNegInf, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
+        for (int c0 = share; c0 < nch; c0 += B * P) {
+            float pm[B], pl[B], mb = M;
+            float4 po[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int x = first + 4 * min(c0 + b * P, nch - 1) * PS;
+                const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, x + 4 * D, 0, AUX));
+                pm[b] = ml.x;
+                pl[b] = ml.y;
+                po[b] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(pr, x + 16 * (i % Q), 0, AUX));
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
+            const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+            sum *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const float e = c0 + b * P < nch && pm[b] != kNegInf ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
+                sum = fmaf(e, pl[b], sum);
+                o.x = fmaf(e, po[b].x, o.x); o.y = fmaf(e, po[b].y, o.y); o.z = fmaf(e, po[b].z, o.z); o.w = fmaf(e, po[b].w, o.w);
+            }
+            M = mb;
+        }
+    }
+    if (P > 1) {
+        sm.m[tid] = M;
+        sm.l[tid] = sum;
+        sm.o[tid] = o;
+        __syncthreads();
+        if (share) return;
+        const float m0 = M;
+        for (int k = 1; k < P; ++k) M = fmaxf(M, sm.m[i + k * n]);
+        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+        sum *= f0;
+        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+        for (int k = 1; k < P; ++k) {
+            const float mk = sm.m[i + k * n], f = mk == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mk - M);
+            const float4 x = sm.o[i + k * n];
+            sum = fmaf(f, sm.l[i + k * n], sum);
+            o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+        }
+    }
+    if (!on || share) return;
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    const float x[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
+    __builtin_memcpy(out + at * D + 4 * (i % Q), x, 16);
+}
+
+constexpr int kWaves = 8;   // of a workgroup of 16 rows
+
+template <int D>
+struct Kv4WavesLds {
+    float o[kWaves][16 * (D + 4)], m[kWaves][16], l[kWaves][16], f[kWaves][16];
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
+    constexpr int NB = D / 32, NG = 1, ROWS = 16 * NG, OS = D + 4;
     __shared__ int last;
-    __shared__ __align__(16) float os[kWaves][ROWS * OS];
-    __shared__ float ms[kWaves][ROWS], ls[kWaves][ROWS];
+    __shared__ __align__(16) union Lds {   // the chunks are merged after the waves
+        Kv4WavesLds<D> waves;
+        Kv4MergeLds<D> merge;
+    } lds;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
     const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, row0 = blockIdx.z * ROWS, R = a.T * a.rep;
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
@@ -543,69 +566,66 @@ __global__ __launch_bounds__(64 * kv4_waves(NG), NG == 1 ? 2 : 1) void kv4_attn_
         }
 
     // ---- the waves' results, then the chunk's ----
+    Kv4WavesLds<D>& x = lds.waves;
+    const float sum = over_groups_sum(r.l[0]);
+    if (L == 0) {
+        x.m[w][c] = sum != sum ? INFINITY : r.m2[0];   // a NaN has to win where the others' weights would drop it
+        x.l[w][c] = sum;
+    }
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-        const float sum = over_groups_sum(r.l[n]);
-        if (L == 0) {
-            ms[w][16 * n + c] = sum != sum ? INFINITY : r.m2[n];   // a NaN has to win where the others' weights would drop it
-            ls[w][16 * n + c] = sum;
-        }
+    for (int b = 0; b < NB; ++b)   // rows 4L + j of the two tiles: elements 8L + 2j and 8L + 2j + 1 of the block
 #pragma unroll
-        for (int b = 0; b < NB; ++b)   // rows 4L + j of the two tiles: elements 8L + 2j and 8L + 2j + 1 of the block
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float4*>(&x.o[w][c * OS + 32 * b + 8 * L + 4 * h]) =
+                make_float4(r.o[0][2 * b][2 * h], r.o[0][2 * b + 1][2 * h], r.o[0][2 * b][2 * h + 1], r.o[0][2 * b + 1][2 * h + 1]);
+    __syncthreads();
+    const int rows = min(ROWS, R - row0), tid = threadIdx.x;
+    if (tid < 16 * kWaves) {
+        const int k = tid >> 4, j = tid & 15;
+        float M = x.m[0][j];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<float4*>(&os[w][(16 * n + c) * OS + 32 * b + 8 * L + 4 * h]) =
-                    make_float4(r.o[n][2 * b][2 * h], r.o[n][2 * b + 1][2 * h], r.o[n][2 * b][2 * h + 1], r.o[n][2 * b + 1][2 * h + 1]);
+        for (int i = 1; i < kWaves; ++i) M = fmaxf(M, x.m[i][j]);
+        x.f[k][j] = x.m[k][j] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.m[k][j] - M);
     }
     __syncthreads();
-    const int rows = min(ROWS, R - row0);
-    for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) {
-        const int k0 = i / D, e = i - k0 * D;
-        float M = ms[0][k0], sum = 0.f, x = 0.f;
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) M = fmaxf(M, ms[k][k0]);
+    for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
+        const int j = i / (D / 4), e = 4 * (i % (D / 4));
+        float M = x.m[0][j], l = 0.f, v[4] = {};
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            const float f = ms[k][k0] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms[k][k0] - M);
-            sum += f * ls[k][k0];
-            x += f * os[k][k0 * OS + e];
+            const float f = x.f[k][j];
+            const float4 y = *reinterpret_cast<const float4*>(&x.o[k][j * OS + e]);
+            M = fmaxf(M, x.m[k][j]);
+            l = fmaf(f, x.l[k][j], l);
+            v[0] = fmaf(f, y.x, v[0]); v[1] = fmaf(f, y.y, v[1]); v[2] = fmaf(f, y.z, v[2]); v[3] = fmaf(f, y.w, v[3]);
         }
-        const size_t at = kv4_q_row(a, g, row0 + k0);
+        const size_t at = kv4_q_row(a, g, row0 + j);
         if (nch == 1) {
-            a.out[at * D + e] = sum == 0.f ? 0.f : x / sum;
+            const float by = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] *= by;
+            __builtin_memcpy(a.out + at * D + e, v, 16);
             continue;
         }
-        float* p = a.part + (at * nch + chunk) * (D + 2);
-        if (a.ctr) {   // read by another workgroup of this launch
-            __hip_atomic_store(p + e, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (e == 0) {
-                __hip_atomic_store(p + D, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(p + D + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        } else {
-            p[e] = x;
-            if (e == 0) {
-                p[D] = M;
-                p[D + 1] = sum;
-            }
-        }
+        // Past this die's L2 (sc1): read by another workgroup of this launch.
+        const int p = (int)(4 * ((at * nch + chunk) * kv4_part(D) + e));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4v, make_float4(v[0], v[1], v[2], v[3])), part_buffer(a.part), p, 0, 16);
+        if (e == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2v, make_float2(M, l)), part_buffer(a.part), p + 4 * D, 0, 16);
     }
     if (nch == 1 || !a.ctr) return;
 
     // ---- the workgroup that comes last merges the block's chunks, in their order ----
     __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's stores acknowledged (vmcnt 0)
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         int* ctr = a.ctr + (size_t)(blockIdx.z * gridDim.y + g) * kSmallTileCtrStride;
         last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nch - 1;
         if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!last) return;
-    for (int i = w; i < rows; i += kWaves) {
-        const size_t at = kv4_q_row(a, g, row0 + i);
-        kv4_merge_row<D, 1, true>(a.part + at * nch * (D + 2), nch, 0, lane, a.out + at * D, nullptr, nullptr, nullptr);
-    }
+    kv4_merge<D, true>(lds.merge, a.part, nch, rows, a.out, [&](int j) { return kv4_q_row(a, g, row0 + j); });
 }
 
 // ---- many rows --------------------------------------------------------------------
@@ -649,17 +669,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     constexpr int PAIRS = Stage::GROUPS / 2;
     __shared__ Stage stage[2];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
-    const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, R = a.T * a.rep, past = a.ctx - a.T + 1;
+    const int g = blockIdx.x, R = a.T * a.rep, past = a.ctx - a.T + 1;
     // The first workgroups, one a CU, take the longest rows from the last block down; the
     // others the shortest ones up.
-    const int nblk = gridDim.z, ahead = min(nblk, (256 + nch * (int)gridDim.y - 1) / (nch * (int)gridDim.y)), z = blockIdx.z;
-    const int block = z < ahead ? nblk - 1 - z : z - ahead;
+    const int nblk = gridDim.y, ahead = min(nblk, (256 + (int)gridDim.x - 1) / (int)gridDim.x), y = blockIdx.y;
+    const int block = y < ahead ? nblk - 1 - y : y - ahead;
     const int row0 = block * kTileRows + ROWS * w;
     auto keys_of = [&](int row) { return past + kv4_token(a, min(row, R - 1)); };
     const int most = row0 < R ? keys_of(row0 + ROWS - 1) : 0;
-    const int s0 = chunk * a.rounds;
-    const int s1 = min(s0 + a.rounds, (keys_of(block * kTileRows + kTileRows - 1) + Stage::KEYS - 1) / Stage::KEYS);
-    const int inside = min(s1, keys_of(block * kTileRows) / Stage::KEYS);   // stages below it are whole for every row
+    const int end = (keys_of(block * kTileRows + kTileRows - 1) + Stage::KEYS - 1) / Stage::KEYS;
+    const int inside = keys_of(block * kTileRows) / Stage::KEYS;   // stages below it are whole for every row
 
     // This wave's runs of a stage: 1 KiB of K, of V, and (lanes 0..15) half of the scales of K (waves 0, 1) or V.
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
@@ -725,7 +744,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     Kv4Rows<NB, NG> r;
     kv4_rows_init<NB, NG>(r, a, g, min(row0, R - 1), R, c, L);
     bool left = false;
-    stages(s0, inside, [&](const Stage& st, int s) {
+    stages(0, inside, [&](const Stage& st, int s) {
         if (is_large(st)) {
             left = true;
             return;
@@ -734,7 +753,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         for (int i = 0; i < PAIRS; ++i)
             kv4_keys<kInside, 2>(r, Kv4FromStage<NB>{st, 2 * i, lane}, s * Stage::KEYS + 64 * i, L);
     });
-    stages(max(s0, inside), s1, [&](const Stage& st, int s) {
+    stages(inside, end, [&](const Stage& st, int s) {
         if (is_large(st)) {
             left = true;
             return;
@@ -746,7 +765,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         }
     });
     if (left)
-        stages(s0, s1, [&](const Stage& st, int s) {
+        stages(0, end, [&](const Stage& st, int s) {
             if (!is_large(st)) return;
 #pragma unroll 1
             for (int i = 0; i < Stage::GROUPS; ++i) {
@@ -760,31 +779,23 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         const int row = row0 + 16 * n + c;
         if (row >= R) continue;
         const size_t at = kv4_q_row(a, g, row);
-        float* to = nch == 1 ? a.out + at * D : a.part + (at * nch + chunk) * (D + 2);
-        const float by = nch > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const float by = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float x[4] = {r.o[n][2 * b][2 * h] * by, r.o[n][2 * b + 1][2 * h] * by, r.o[n][2 * b][2 * h + 1] * by,
                                     r.o[n][2 * b + 1][2 * h + 1] * by};
-                __builtin_memcpy(to + 32 * b + 8 * L + 4 * h, x, 16);
+                __builtin_memcpy(a.out + at * D + 32 * b + 8 * L + 4 * h, x, 16);
             }
-        if (nch > 1 && L == 0) {
-            to[D] = sum != sum ? INFINITY : r.m2[n];
-            to[D + 1] = sum;
-        }
     }
 }
 
-// The merge as a launch of its own: W waves a row, eight a workgroup.
-template <int D, int W>
-__global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, int rows,
-                                                        float* __restrict__ out) {
-    __shared__ float sm[8], sl[8], so[8][D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = (int)blockIdx.x * (8 / W) + wave / W;
-    if (W == 1 && row >= rows) return;   // W 8: a row a workgroup
-    kv4_merge_row<D, W, false>(part + (size_t)row * nch * (D + 2), nch, wave % W, lane, out + (size_t)row * D, sm, sl, so);
+// The merge as a launch of its own: a row a workgroup.
+template <int D>
+__global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, float* __restrict__ out) {
+    __shared__ Kv4MergeLds<D> sm;
+    kv4_merge<D, false>(sm, part, nch, 1, out, [](int) { return (size_t)blockIdx.x; });
 }
 
 }  // namespace
@@ -815,40 +826,30 @@ int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, in
 
 namespace {
 struct Kv4Plan {
-    int groups = 1;                          // 16-row groups a block of the rows kernel; 0: the tiles kernel
+    bool tiles = false;                      // the kernel for many rows
     int blocks = 1, rounds = 1, nch = 1;     // blocks of rows of a KV head
 };
 
-Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
+Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
     Kv4Plan p;
     const long R = (long)T * (n_heads / n_kv);
-    const char* e = std::getenv("KV4_TILES");
-    const long from = e ? atol(e) : 64;
-    if (R >= from) {
-        const long nb = (ctx_len + 8192 / d_head - 1) / (8192 / d_head), want = 512;   // stages, workgroups
-        p.groups = 0;
-        p.blocks = (int)((R + kTileRows - 1) / kTileRows);
-        long nch = std::max(1l, want / ((long)p.blocks * n_kv));
-        nch = std::min(nch, nb);
-        p.rounds = (int)((nb + nch - 1) / nch);
-        p.nch = (int)((nb + p.rounds - 1) / p.rounds);
+    p.blocks = (int)((R + kTileRows - 1) / kTileRows);
+    if ((long)p.blocks * n_kv >= (std::getenv("KV4_TILES") ? atol(std::getenv("KV4_TILES")) : 240)) {
+        p.tiles = true;
         return p;
     }
-    p.groups = R > 16 ? 2 : 1;
-    if (const char* f = std::getenv("KV4_G")) p.groups = atoi(f);
-    p.blocks = (int)((R + 16 * p.groups - 1) / (16 * p.groups));
-    const long nb = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
-    const long waves = kv4_waves(p.groups), want = 2048 / waves;
-    p.rounds = (int)((nb * p.blocks * n_kv + waves * want - 1) / (waves * want));
-    p.nch = (int)((nb + waves * p.rounds - 1) / (waves * p.rounds));
+    p.blocks = (int)((R + 15) / 16);
+    const long nb = (ctx_len + kv4::kKeys - 1) / kv4::kKeys, want = std::getenv("KV4_WANT") ? atol(std::getenv("KV4_WANT")) : 2048;
+    p.rounds = (int)((nb * p.blocks * n_kv + want - 1) / want);
+    p.nch = (int)((nb + kWaves * p.rounds - 1) / (kWaves * p.rounds));
     return p;
 }
 }  // namespace
 
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1) return 0;   // refused by the launch
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
-    return p.nch > 1 ? (size_t)T * n_heads * p.nch * (d_head + 2) * sizeof(float) : 0;
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    return p.nch > 1 ? (size_t)T * n_heads * p.nch * kv4_part(d_head) * sizeof(float) : 0;
 }
 
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
@@ -858,10 +859,10 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     VH_ARG(ctx_len >= 1 && ctx_len <= max_seq && T >= 1 && T <= ctx_len, "attn: %d rows of %d keys in a cache of %d", T,
            ctx_len, max_seq);
     VH_ARG((long)T * n_heads < (1l << 31), "attn: %d rows of %d heads", T, n_heads);
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
     VH_ARG(p.blocks <= 65535 && n_kv <= 65535 && (size_t)T * n_heads / n_kv * (n_heads / n_kv) < (1ull << 32),
            "attn: %d rows of %d heads over %d KV heads are beyond a launch", T, n_heads, n_kv);
-    VH_ARG(p.nch == 1 || part, "attn: no scratch");
+    VH_ARG(p.nch == 1 || (part && attn_kv4_part_bytes(n_heads, n_kv, d_head, T, ctx_len) < (1ull << 31)), "attn: no scratch");
     Kv4Attn a;
     a.q = q;
     a.kc = reinterpret_cast<const uint8_t*>(L.k);
@@ -870,7 +871,7 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     a.vs = reinterpret_cast<const uint16_t*>(L.vs);
     a.out = out;
     a.part = part;
-    const bool merged = ctr && p.groups == 1 && (long)p.blocks * n_kv <= kSmallMaxTiles && p.nch <= 32;
+    const bool merged = ctr && (long)p.blocks * n_kv <= kSmallMaxTiles && p.nch <= (std::getenv("KV4_M") ? atoi(std::getenv("KV4_M")) : 32);
     a.ctr = merged ? ctr : nullptr;
     a.codes = kv4::head_codes(max_seq, d_head);
     a.scales = kv4::head_scales(max_seq, d_head);
@@ -884,32 +885,20 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     // Never 0: a masked score's -inf times the factor has to stay -inf.
     a.sl2 = std::max((float)(std::fabs((double)scale) * 1.4426950408889634), 1e-20f);
     a.qsign = scale < 0.f ? -1.f : 1.f;
-    const dim3 grid(p.nch, n_kv, p.blocks);
-#define VH_ROWS(D, G) VH_LAUNCH((kv4_attn_rows_kernel<D, G>), grid, dim3(64 * kv4_waves(G)), 0, s, a)
-    if (p.groups == 0) {
+    if (p.tiles) {
+        const dim3 grid(n_kv, p.blocks);
         if (d_head == 64) VH_LAUNCH(kv4_attn_tiles_kernel<64>, grid, dim3(64 * kTileWaves), 0, s, a);
         else VH_LAUNCH(kv4_attn_tiles_kernel<128>, grid, dim3(64 * kTileWaves), 0, s, a);
-    } else if (d_head == 64) {
-        if (p.groups == 1) VH_ROWS(64, 1);
-        else VH_ROWS(64, 2);
-    } else {
-        if (p.groups == 1) VH_ROWS(128, 1);
-        else VH_ROWS(128, 2);
+        VH_LAUNCHED();
+        return VLRF_HIP_OK;
     }
-#undef VH_ROWS
+    const dim3 grid(p.nch, n_kv, p.blocks);
+    if (d_head == 64) VH_LAUNCH(kv4_attn_rows_kernel<64>, grid, dim3(64 * kWaves), 0, s, a);
+    else VH_LAUNCH(kv4_attn_rows_kernel<128>, grid, dim3(64 * kWaves), 0, s, a);
     VH_LAUNCHED();
     if (p.nch == 1 || merged) return VLRF_HIP_OK;
-    const int rows = T * n_heads;
-#define VH_MERGE(D, W) \
-    VH_LAUNCH((kv4_merge_kernel<D, W>), dim3((rows + 8 / W - 1) / (8 / W)), dim3(512), 0, s, part, p.nch, rows, out)
-    if (d_head == 64) {
-        if (p.nch <= 8) VH_MERGE(64, 1);
-        else VH_MERGE(64, 8);
-    } else {
-        if (p.nch <= 8) VH_MERGE(128, 1);
-        else VH_MERGE(128, 8);
-    }
-#undef VH_MERGE
+    if (d_head == 64) VH_LAUNCH(kv4_merge_kernel<64>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out);
+    else VH_LAUNCH(kv4_merge_kernel<128>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out);
     VH_LAUNCHED();
     return VLRF_HIP_OK;
 }
