@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 namespace vlrf_hip {
 namespace {
@@ -162,6 +163,14 @@ __device__ __forceinline__ void split2(float x, float f, float y, float g, h2v& 
     lo = h2v{(_Float16)fmaf(x, f, -(float)hi.x), (_Float16)fmaf(y, g, -(float)hi.y)};
 }
 
+// The same of single values.
+__device__ __forceinline__ void split2(float x, float y, h2v& hi, h2v& lo) {
+    uint32_t h = __builtin_bit_cast(uint32_t, h2v{(_Float16)x, (_Float16)y});
+    asm("" : "+v"(h));
+    hi = as_h2(h);
+    lo = h2v{(_Float16)(x - (float)hi.x), (_Float16)(y - (float)hi.y)};
+}
+
 __device__ __forceinline__ float over_groups_max(float v) {   // over the lanes of a column
     float2 t = swap_rows16(v, v);
     v = fmaxf(t.x, t.y);
@@ -302,6 +311,36 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
 
     __builtin_amdgcn_sched_barrier(0);
     // ---- output ----
+    if constexpr (Src::kValues && MODE != kApart) {
+        // Whole values stand in two pieces: p alone is split, once for all blocks.
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) {
+            h8v ph[NG], pl[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                h2v hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * (i >> 1) + (i & 1);
+                    split2(s[kg][n][e], s[kg][n][e + 2], hi[i], lo[i]);
+                }
+                ph[n] = h8_of(hi[0], hi[1], hi[2], hi[3]);
+                pl[n] = h8_of(lo[0], lo[1], lo[2], lo[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * NB; ++t) {
+                h8v vh, vl;
+                src.value(kg, t, vh, vl);
+#pragma unroll
+                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[n], r.o[n][t], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[n], r.o[n][t], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[n], r.o[n][t], 0, 0, 0);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
@@ -365,7 +404,9 @@ struct Kv4Raw {
     uint32_t kw[2][NB], vw[2 * NB];
     uint4 kd[NB], vd[NB];
     uint32_t magic;
+    static constexpr bool kValues = false;
 
+    __device__ __forceinline__ void value(int, int, h8v&, h8v&) const {}
     __device__ __forceinline__ h8v k(int, int u, int b) const {
         h2v x0, x1, x2, x3;
         codes8(kw[u][b], magic, x0, x1, x2, x3);
@@ -631,30 +672,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
 // ---- many rows --------------------------------------------------------------------
 // Four waves of 32 rows share what they read: a stage of 8192 / D keys is decoded once,
 // into LDS, where the operands stand as the lanes read them (a wave decodes a quarter of
-// the stage's K and of its V).  Stages alternate between two buffers, one barrier a
-// stage; the next one's codes are in registers meanwhile.  Each wave keeps its rows to
-// the end, so nothing is merged but chunks of keys where there are few rows.  Three
-// passes over the stages, as above.
+// the stage's K and of its V).  The next stage's codes are in registers meanwhile; the
+// other workgroup of the CU computes while this one decodes.  Values stand whole, as two
+// f16 pieces whose sum is exactly the code times the scale (15 bits) while the scale is
+// below 8192, so that only p is split, once for all blocks: three products for two, but
+// a quarter of the conversions, which cost more (16 cycles a weight and block).  Stages
+// with a larger scale, or one that is no number, come last, with codes and scales apart.
+// Each wave keeps its rows to the end, so nothing is merged.  Three passes, as above.
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 
 template <int NB>
 struct Kv4Stage {
     static constexpr int GROUPS = 8 / NB, KEYS = 32 * GROUPS;
-    uint4 k[16][64], v[16][64];    // [group][2 NB][lane]
-    uint4 kd[32], vd[32];          // [group][L][block]
-    uint32_t large[2];             // a scale of 2 or more among a half of vd
+    uint4 k[16][64];               // [group][2][NB][lane]
+    uint4 v[2][16][64];            // pieces of [group][NB][2][lane]; apart: codes in the first
+    uint4 kd[32], vd[32];          // [group][L][block]; vd: apart only
+    uint32_t large[kTileWaves];    // a scale of 8192 or more among the wave's values
 };
 
 template <int NB>
 struct Kv4FromStage {
     const Kv4Stage<NB>& st;
     int group, lane;
+    static constexpr bool kValues = true;
     __device__ __forceinline__ h8v k(int kg, int u, int b) const {
         return __builtin_bit_cast(h8v, st.k[(2 * (group + kg) + u) * NB + b][lane]);
     }
+    __device__ __forceinline__ void value(int kg, int t, h8v& hi, h8v& lo) const {
+        hi = __builtin_bit_cast(h8v, st.v[0][2 * (group + kg) * NB + t][lane]);
+        lo = __builtin_bit_cast(h8v, st.v[1][2 * (group + kg) * NB + t][lane]);
+    }
     __device__ __forceinline__ void v(int kg, int b, h8v& even, h8v& odd) const {
-        even = __builtin_bit_cast(h8v, st.v[2 * ((group + kg) * NB + b)][lane]);
-        odd = __builtin_bit_cast(h8v, st.v[2 * ((group + kg) * NB + b) + 1][lane]);
+        even = __builtin_bit_cast(h8v, st.v[0][2 * ((group + kg) * NB + b)][lane]);
+        odd = __builtin_bit_cast(h8v, st.v[0][2 * ((group + kg) * NB + b) + 1][lane]);
     }
     __device__ __forceinline__ uint2 ks(int kg, int u, int b) const {
         return reinterpret_cast<const uint2*>(&st.kd[(4 * (group + kg) + (lane >> 4)) * NB + b])[u];
@@ -667,7 +717,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     constexpr int NB = D / 32, NG = 2, ROWS = 16 * NG;
     using Stage = Kv4Stage<NB>;
     constexpr int PAIRS = Stage::GROUPS / 2;
-    __shared__ Stage stage[2];
+    __shared__ Stage st;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
     const int g = blockIdx.x, R = a.T * a.rep, past = a.ctx - a.T + 1;
     // The first workgroups, one a CU, take the longest rows from the last block down; the
@@ -680,72 +730,92 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     const int end = (keys_of(block * kTileRows + kTileRows - 1) + Stage::KEYS - 1) / Stage::KEYS;
     const int inside = keys_of(block * kTileRows) / Stage::KEYS;   // stages below it are whole for every row
 
-    // This wave's runs of a stage: 1 KiB of K, of V, and (lanes 0..15) half of the scales of K (waves 0, 1) or V.
+    // This wave's runs of a stage: 1 KiB of K and of V (two blocks of a group of keys), the
+    // scales of those values, and (lanes 0..7) a quarter of K's.
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
     const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
     const uint32_t magic = magic1024();
+    const int vgroup = D == 64 ? w : w >> 1, vblock = D == 64 ? 0 : 2 * (w & 1);
     uint32_t kw[4], vw[4];
-    uint4 sc;
+    uint4 kd, vd[2];
     auto fetch = [&](int s) {   // past the cache's end: zeros
         const size_t at = (size_t)s * 4096, sat = (size_t)s * 256;   // bytes of codes, f16 scales
         const int left = (int)min((size_t)4096, a.codes - at), sleft = (int)min((size_t)256, a.scales - sat) * 2;
         const auto kr = group_buffer(kc + at, left), vr = group_buffer(vc + at, left);
+        const auto sr = group_buffer(ks + sat, sleft), tr = group_buffer(vs + sat, sleft);
         if constexpr (D == 64) {   // a run of K holds both halves of a group's keys, 8 bytes a lane
             uint32_t x[2], y[2];
             buffer_words<2>(x, kr, 1024 * w + c * 32 + 8 * L);
             buffer_words<2>(y, kr, 1024 * w + (c + 16) * 32 + 8 * L);
             kw[0] = x[0]; kw[1] = x[1]; kw[2] = y[0]; kw[3] = y[1];
-            buffer_words<4>(vw, vr, 1024 * w + (L * 16 + c) * 16);
         } else {
             buffer_words<4>(kw, kr, 1024 * w + c * 64 + 16 * L);
-            buffer_words<4>(vw, vr, 2048 * (w >> 1) + (L * 16 + c) * 32 + 16 * (w & 1));
         }
-        const auto sr = group_buffer((w & 2) ? vs + sat : ks + sat, sleft);
-        sc = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (16 * (w & 1) + c), 0, 0));
+        buffer_words<4>(vw, vr, 32 * (D / 2) * vgroup + (L * 16 + c) * 8 * NB + 8 * vblock);
+        kd = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (8 * w + (lane & 7)), 0, 0));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            vd[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * ((4 * vgroup + L) * NB + vblock + j), 0, 0));
     };
-    auto put = [&](Stage& st) {
+    auto put = [&](auto apart) {
         h2v x0, x1, x2, x3, y0, y1, y2, y3;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             codes8(kw[j], magic, x0, x1, x2, x3);
             st.k[4 * w + j][lane] = __builtin_bit_cast(uint4, h8_of(x0, x1, x2, x3));
         }
+        uint32_t big = 0;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             codes8(vw[2 * j], magic, x0, x1, x2, x3);
             codes8(vw[2 * j + 1], magic, y0, y1, y2, y3);
-            st.v[4 * w + 2 * j][lane] = __builtin_bit_cast(uint4, h8_of(x0, x2, y0, y2));
-            st.v[4 * w + 2 * j + 1][lane] = __builtin_bit_cast(uint4, h8_of(x1, x3, y1, y3));
+            const int t = 4 * w + 2 * j;   // even elements; odd ones in t + 1
+            if constexpr (decltype(apart)::value) {
+                st.v[0][t][lane] = __builtin_bit_cast(uint4, h8_of(x0, x2, y0, y2));
+                st.v[0][t + 1][lane] = __builtin_bit_cast(uint4, h8_of(x1, x3, y1, y3));
+                if (c == 0) st.vd[(4 * vgroup + L) * NB + vblock + j] = vd[j];
+            } else {
+                // The scales of slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.
+                const h2v d0 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x05040100)), d1 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x07060302));
+                const h2v d2 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x05040100)), d3 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x07060302));
+                auto both = [&](int to, h2v a0, h2v a1, h2v a2, h2v a3) {
+                    const h2v h0 = a0 * d0, h1 = a1 * d1, h2 = a2 * d2, h3 = a3 * d3;
+                    st.v[0][to][lane] = __builtin_bit_cast(uint4, h8_of(h0, h1, h2, h3));
+                    st.v[1][to][lane] = __builtin_bit_cast(uint4, h8_of(__builtin_elementwise_fma(a0, d0, -h0), __builtin_elementwise_fma(a1, d1, -h1),
+                                                                        __builtin_elementwise_fma(a2, d2, -h2), __builtin_elementwise_fma(a3, d3, -h3)));
+                };
+                both(t, x0, x2, y0, y2);
+                both(t + 1, x1, x3, y1, y3);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {   // exponent bits 111xx: 8192 and more
+                const uint32_t x = word_of(vd[j], i);
+                big |= x & (x << 1) & (x << 2);
+            }
         }
-        if (lane < 16) ((w & 2) ? st.vd : st.kd)[16 * (w & 1) + lane] = sc;
-        const bool big = __builtin_amdgcn_ballot_w64(((sc.x | sc.y | sc.z | sc.w) & 0x40004000u) != 0) != 0;
-        if (lane == 0 && (w & 2)) st.large[w & 1] = big;
+        if (lane < 8) st.kd[8 * w + lane] = kd;
+        const bool any = __builtin_amdgcn_ballot_w64((big & 0x40004000u) != 0) != 0;
+        if (lane == 0) st.large[w] = any;
     };
-    // The stages [from, to): body(stage, s) with each one in LDS.
-    auto stages = [&](int from, int to, auto body) {
+    // The stages [from, to): body(s) with each one in LDS.
+    auto stages = [&](auto apart, int from, int to, auto body) {
         if (from >= to) return;
         fetch(from);
-        put(stage[0]);
-        if (from + 1 < to) fetch(from + 1);
-        __syncthreads();
         for (int s = from; s < to; ++s) {
-            body(stage[(s - from) & 1], s);
-            if (s + 1 < to) {   // into the buffer of stage s - 1: every wave is past its barrier
-                put(stage[(s + 1 - from) & 1]);
-                if (s + 2 < to) fetch(s + 2);
-            }
+            __syncthreads();   // every wave has read the stage before
+            put(apart);
+            if (s + 1 < to) fetch(s + 1);
             __syncthreads();
+            body(s);
         }
     };
-    auto is_large = [&](const Stage& st) {
-        return __builtin_amdgcn_readfirstlane(st.large[0] | st.large[1]) != 0;
-    };
+    auto is_large = [&]() { return __builtin_amdgcn_readfirstlane(st.large[0] | st.large[1] | st.large[2] | st.large[3]) != 0; };
 
     Kv4Rows<NB, NG> r;
     kv4_rows_init<NB, NG>(r, a, g, min(row0, R - 1), R, c, L);
     bool left = false;
-    stages(0, inside, [&](const Stage& st, int s) {
-        if (is_large(st)) {
+    stages(std::false_type(), 0, inside, [&](int s) {
+        if (is_large()) {
             left = true;
             return;
         }
@@ -753,8 +823,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         for (int i = 0; i < PAIRS; ++i)
             kv4_keys<kInside, 2>(r, Kv4FromStage<NB>{st, 2 * i, lane}, s * Stage::KEYS + 64 * i, L);
     });
-    stages(inside, end, [&](const Stage& st, int s) {
-        if (is_large(st)) {
+    stages(std::false_type(), inside, end, [&](int s) {
+        if (is_large()) {
             left = true;
             return;
         }
@@ -765,8 +835,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         }
     });
     if (left)
-        stages(0, end, [&](const Stage& st, int s) {
-            if (!is_large(st)) return;
+        stages(std::true_type(), 0, end, [&](int s) {
+            if (!is_large()) return;
 #pragma unroll 1
             for (int i = 0; i < Stage::GROUPS; ++i) {
                 const int key0 = s * Stage::KEYS + 32 * i;
