@@ -242,37 +242,43 @@ enum { kInside, kEdge, kApart };
 template <int MODE, int KG, int NB, int NG, class Src>
 __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int key0, int L) {
     // ---- scores: slots 4u + j of the lane's keys ----
+    // The next half group's operands are read before this one's products (LDS takes longer
+    // than a few of those); the barriers hold the order.
     float s[KG][NG][8];
+    h8v ka[2][NB];
+    h2v dk[2][NB][2];
+    auto read = [&](int i) {   // half group i
 #pragma unroll
-    for (int kg = 0; kg < KG; ++kg)
+        for (int b = 0; b < NB; ++b) ka[i & 1][b] = src.k(i >> 1, i & 1, b);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            h8v ka[NB];
-            h2v dk[NB][2];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) ka[b] = src.k(kg, u, b);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint2 ks = src.ks(kg, u, b);
-                dk[b][0] = as_h2(ks.x);
-                dk[b][1] = as_h2(ks.y);
-            }
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                f4v t[NB];
-#pragma unroll
-                for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[b], r.ql[n][b], f4v{}, 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[b], r.qh[n][b], t[b], 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float& x = s[kg][n][4 * u + j];
-                        x = fmaf(t[b][j], (float)((j & 1) ? dk[b][j >> 1].y : dk[b][j >> 1].x), b == 0 ? 0.f : x);
-                    }
-            }
+        for (int b = 0; b < NB; ++b) {
+            const uint2 ks = src.ks(i >> 1, i & 1, b);
+            dk[i & 1][b][0] = as_h2(ks.x);
+            dk[i & 1][b][1] = as_h2(ks.y);
         }
+    };
+    read(0);
+#pragma unroll
+    for (int i = 0; i < 2 * KG; ++i) {
+        if (i + 1 < 2 * KG) read(i + 1);
+        if (Src::kValues) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            f4v t[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i & 1][b], r.ql[n][b], f4v{}, 0, 0, 0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) t[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i & 1][b], r.qh[n][b], t[b], 0, 0, 0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float& x = s[i >> 1][n][4 * (i & 1) + j];
+                    const h2v d = dk[i & 1][b][j >> 1];
+                    x = fmaf(t[b][j], (float)((j & 1) ? d.y : d.x), b == 0 ? 0.f : x);
+                }
+        }
+    }
 
     __builtin_amdgcn_sched_barrier(0);   // no loads of the next part early: they would cost registers
     // ---- softmax ----
@@ -313,31 +319,34 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
     // ---- output ----
     if constexpr (Src::kValues && MODE != kApart) {
         // Whole values stand in two pieces: p alone is split, once for all blocks.
+        constexpr int T = 2 * NB, AHEAD = 2;
+        h8v ph[KG][NG], pl[KG][NG], vh[AHEAD + 1], vl[AHEAD + 1];
+        auto split = [&](int kg, int n) {
+            h2v hi[4], lo[4];
 #pragma unroll
-        for (int kg = 0; kg < KG; ++kg) {
-            h8v ph[NG], pl[NG];
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                h2v hi[4], lo[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 4 * (i >> 1) + (i & 1);
-                    split2(s[kg][n][e], s[kg][n][e + 2], hi[i], lo[i]);
-                }
-                ph[n] = h8_of(hi[0], hi[1], hi[2], hi[3]);
-                pl[n] = h8_of(lo[0], lo[1], lo[2], lo[3]);
+            for (int i = 0; i < 4; ++i) {
+                const int e = 4 * (i >> 1) + (i & 1);
+                split2(s[kg][n][e], s[kg][n][e + 2], hi[i], lo[i]);
             }
+            ph[kg][n] = h8_of(hi[0], hi[1], hi[2], hi[3]);
+            pl[kg][n] = h8_of(lo[0], lo[1], lo[2], lo[3]);
+        };
 #pragma unroll
-            for (int t = 0; t < 2 * NB; ++t) {
-                h8v vh, vl;
-                src.value(kg, t, vh, vl);
+        for (int i = 0; i < AHEAD; ++i) src.value(i / T, i % T, vh[i], vl[i]);
 #pragma unroll
-                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[n], r.o[n][t], 0, 0, 0);
+        for (int n = 0; n < NG; ++n) split(0, n);
 #pragma unroll
-                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[n], r.o[n][t], 0, 0, 0);
+        for (int i = 0; i < KG * T; ++i) {
+            const int kg = i / T, t = i % T, at = i % (AHEAD + 1), next = (i + AHEAD) % (AHEAD + 1);
+            if (i + AHEAD < KG * T) src.value((i + AHEAD) / T, (i + AHEAD) % T, vh[next], vl[next]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[n], r.o[n][t], 0, 0, 0);
-            }
+            for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[at], ph[kg][n], r.o[n][t], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[at], pl[kg][n], r.o[n][t], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) r.o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[at], ph[kg][n], r.o[n][t], 0, 0, 0);
+            if (kg + 1 < KG && t < NG) split(kg + 1, t);   // the next group's weights between this one's products
         }
         return;
     }
