@@ -37,50 +37,132 @@ __device__ __forceinline__ float kv4_inverse(uint32_t d16) {
     return d != 0.f ? 1.f / d : 0.f;
 }
 
-// One thread a block.
-__global__ __launch_bounds__(256) void kv4_append_kernel(uint8_t* kc, uint8_t* vc, uint16_t* ks, uint16_t* vs,
-                                                         const float* __restrict__ k, const float* __restrict__ v,
-                                                         int n_kv, int D, int max_seq, int T, int pos) {
-    const int nb = D / 32;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)T * n_kv * nb;
-    if (i >= 2 * n) return;
-    const bool isv = i >= n;
-    const size_t j = isv ? i - n : i;
-    const int b = (int)(j % nb), g = (int)(j / nb % n_kv), t = pos + (int)(j / nb / n_kv);
-    const float* x = (isv ? v : k) + 32 * j;
-    float e[32], amax = 0.f, m = 0.f;
+// Appending.  A workgroup takes CB blocks of 32 elements of one head's K or V rows at a
+// group of 32 key positions (group kb0 + blockIdx.x), a thread eight elements of a row:
+// the four lanes of a block find its extreme by quad exchanges, and each has a word of
+// codes.  K's words go out as they are, a row's side by side.  V's bytes and the scales
+// are turned in LDS, where a whole group's are side by side, and go out in words; of a
+// group that the rows fill in part, byte by byte, so that the others stay.
+// Bound by the rows' bytes.
+struct Kv4Append {
+    const float *k, *v;       // [T][ld]
+    uint8_t *kc, *vc;
+    uint16_t *ks, *vs;
+    int ld, D, max_seq, T, pos;
+};
+
+__device__ __forceinline__ float quad_f(float v, int which) {   // the lane 1 or 2 away within its four
+    return which == 1 ? dpp_f<0xB1>(v) : dpp_f<0x4E>(v);
+}
+
+template <int CB>
+__global__ __launch_bounds__(128 * CB) void kv4_append_kernel(Kv4Append a) {
+    __shared__ uint32_t codes[128 * CB];
+    __shared__ uint16_t scales[32 * CB];
+    const int tid = threadIdx.x, bl = tid % (4 * CB) / 4, word = tid % 4, slot_key = tid / (4 * CB);
+    const bool isv = blockIdx.z & 1;
+    const int nb = a.D / 32, b = (int)(blockIdx.z >> 1) * CB + bl, g = blockIdx.y;
+    const int kb = a.pos / kv4::kKeys + (int)blockIdx.x, t = kb * kv4::kKeys + slot_key, row = t - a.pos;
+    const bool on = row >= 0 && row < a.T;
+    const bool whole = kb * kv4::kKeys >= a.pos && (kb + 1) * kv4::kKeys <= a.pos + a.T;
+
+    float e[8] = {};
+    if (on) __builtin_memcpy(e, (isv ? a.v : a.k) + (size_t)row * a.ld + g * a.D + 32 * b + 8 * word, 32);
+    // The largest magnitude, the first of equal ones: the maximum of (|x|, -index, sign).
+    float amax = 0.f, m = 0.f;
     bool bad = false;
 #pragma unroll
-    for (int l = 0; l < 32; ++l) {
-        e[l] = x[l];
-        bad |= !(fabsf(e[l]) < INFINITY);
-        if (fabsf(e[l]) > amax) { amax = fabsf(e[l]); m = e[l]; }
+    for (int i = 0; i < 8; ++i) {
+        bad |= !(fabsf(e[i]) < INFINITY);
+        if (fabsf(e[i]) > amax) { amax = fabsf(e[i]); m = e[i]; }
     }
-    const uint32_t d16 = bad ? kNanF16 : kv4_scale_bits(m);
-    const float r = kv4_inverse(d16);
-    (isv ? vs : ks)[g * kv4::head_scales(max_seq, D) + kv4::scale(t, b, D)] = (uint16_t)d16;
-    uint8_t* c = (isv ? vc : kc) + g * kv4::head_codes(max_seq, D);
+    if (bad) m = __uint_as_float(0x7FC00000u);
 #pragma unroll
-    for (int l = 0; l < 16; ++l) {
-        const uint8_t byte = (uint8_t)(kv4_code(e[2 * l], r) | kv4_code(e[2 * l + 1], r) << 4);
-        c[isv ? kv4::v_byte(t, l, b, D) : kv4::k_word(t, l / 4, b, D) + l % 4] = byte;
+    for (int step = 1; step <= 2; ++step) {
+        const float o = quad_f(m, step);
+        const bool below = (word & step) != 0;                       // the other lane's elements come first
+        if (o != o || fabsf(o) > fabsf(m) || (below && fabsf(o) == fabsf(m))) m = o;   // a NaN m loses no comparison
+    }
+    const uint32_t d16 = m != m ? kNanF16 : kv4_scale_bits(m);
+    const float r = kv4_inverse(d16);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= kv4_code(e[i], r) << (4 * i);
+
+    uint8_t* cs = (isv ? a.vc : a.kc) + g * kv4::head_codes(a.max_seq, a.D);
+    uint16_t* ds = (isv ? a.vs : a.ks) + g * kv4::head_scales(a.max_seq, a.D);
+    if (!isv && on) *reinterpret_cast<uint32_t*>(cs + kv4::k_word(t, word, b, a.D)) = w;
+    if (!whole) {
+        if (!on) return;
+        if (isv) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cs[kv4::v_byte(t, 4 * word + i, b, a.D)] = (uint8_t)(w >> (8 * i));
+        }
+        if (word == 0) ds[kv4::scale(t, b, a.D)] = (uint16_t)d16;
+        return;
+    }
+    const int L = kv4::lane_group(t), slot = kv4::slot(t);
+    if (isv) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint8_t*>(codes)[8 * ((L * 16 + 4 * word + i) * CB + bl) + slot] = (uint8_t)(w >> (8 * i));
+    }
+    if (word == 0) scales[8 * (L * CB + bl) + slot] = (uint16_t)d16;
+    __syncthreads();
+    const int b0 = b - bl, t0 = kb * kv4::kKeys;
+    if (isv) {   // word 2 (run * CB + block) + half of the turned codes
+        const int run = tid / (2 * CB), blk = tid / 2 % CB;
+        *reinterpret_cast<uint32_t*>(cs + kv4::v_byte(t0, 0, 0, a.D) + 8 * (run * nb + b0 + blk) + 4 * (tid & 1)) = codes[tid];
+    }
+    if (tid < 16 * CB) {
+        const int grp = tid / (4 * CB), blk = tid / 4 % CB;
+        *reinterpret_cast<uint32_t*>(ds + kv4::scale(t0, 0, a.D) + 8 * (grp * nb + b0 + blk) + 2 * (tid & 3)) =
+            reinterpret_cast<const uint32_t*>(scales)[tid];
     }
 }
 
-// One thread a byte of two codes.
+// Reading back.  A workgroup takes CB blocks of one head at a group of 32 keys: of K a
+// thread four elements of a row at a time, of V a byte of eight keys, halves exchanged
+// between neighbours so that it writes four elements of four keys.  Bound by the bytes
+// that it writes.
+template <int CB>
 __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                           const uint16_t* __restrict__ ks,
-                                                          const uint16_t* __restrict__ vs, int n_kv, int D, int max_seq,
+                                                          const uint16_t* __restrict__ vs, int row, int D, int max_seq,
                                                           int ctx, float* __restrict__ K, float* __restrict__ V) {
-    const int pairs = D / 2;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)ctx * n_kv * pairs;
-    if (i >= n) return;
-    const int p = (int)(i % pairs), g = (int)(i / pairs % n_kv), t = (int)(i / pairs / n_kv), b = p / 16, l = p % 16;
-    const size_t cb = g * kv4::head_codes(max_seq, D), sb = g * kv4::head_scales(max_seq, D) + kv4::scale(t, b, D);
-    const uint32_t kb = kc[cb + kv4::k_word(t, l / 4, b, D) + l % 4], vb = vc[cb + kv4::v_byte(t, l, b, D)];
-    const float kd = f16_bits_to_f32(ks[sb]), vd = f16_bits_to_f32(vs[sb]);
-    reinterpret_cast<float2*>(K)[i] = make_float2((float)((int)(kb & 15u) - 8) * kd, (float)((int)(kb >> 4) - 8) * kd);
-    reinterpret_cast<float2*>(V)[i] = make_float2((float)((int)(vb & 15u) - 8) * vd, (float)((int)(vb >> 4) - 8) * vd);
+    const int nb = D / 32, b0 = blockIdx.z * CB, g = blockIdx.y, t0 = blockIdx.x * kv4::kKeys, tid = threadIdx.x;
+    const size_t cb = g * kv4::head_codes(max_seq, D), sb = g * kv4::head_scales(max_seq, D);
+    auto put = [&](float* to, int t, int e, float4 x) {
+        if (t < ctx) __builtin_memcpy(to + (size_t)t * row + g * D + e, &x, 16);
+    };
+    auto value = [](uint32_t w, int i, float d) { return (float)((int)(w >> (4 * i) & 15u) - 8) * d; };
+    constexpr int KI = 256 * CB;   // items of K: 32 keys, 8 CB times four elements
+#pragma unroll
+    for (int m = tid; m < KI; m += 256) {
+        const int q = m % (8 * CB), t = t0 + m / (8 * CB), b = b0 + q / 8;
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(kc + cb + kv4::k_word(t, q % 8 / 2, b, D)) >> (16 * (q & 1));
+        const float d = f16_bits_to_f32(ks[sb + kv4::scale(t, b, D)]);
+        put(K, t, 32 * b0 + 4 * q, make_float4(value(w, 0, d), value(w, 1, d), value(w, 2, d), value(w, 3, d)));
+    }
+    constexpr int VI = 64 * CB;    // items of V: 4 groups of keys, CB blocks, 16 bytes
+#pragma unroll
+    for (int m = tid; m < VI; m += 256) {
+        const int i = m % 16, bl = m / 16 % CB, L = m / (16 * CB), b = b0 + bl;
+        uint2 x = *reinterpret_cast<const uint2*>(vc + cb + kv4::v_byte(t0, 0, 0, D) + 8 * ((L * 16 + i) * nb + b));
+        const uint4 d = *reinterpret_cast<const uint4*>(vs + sb + kv4::scale(t0, 0, D) + 8 * (L * nb + b));
+        // Even lanes take slots 0..3 of both bytes, odd lanes slots 4..7.
+        const bool odd = i & 1;
+        const uint32_t give = odd ? x.x : x.y, keep = odd ? x.y : x.x;
+        const uint32_t got = __float_as_uint(dpp_f<0xB1>(__uint_as_float(give)));
+        const uint32_t lo = odd ? got : keep, hi = odd ? keep : got;   // bytes of elements 4 (i / 2) .. + 1 and + 2 .. + 3
+        const uint2 dd = odd ? make_uint2(d.z, d.w) : make_uint2(d.x, d.y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t p = lo >> (8 * j), q = hi >> (8 * j);
+            const float s = f16_bits_to_f32(((j & 2) ? dd.y : dd.x) >> (16 * (j & 1)) & 0xFFFFu);
+            put(V, t0 + kv4::key_of(L, (odd ? 4 : 0) + j), 32 * b + 2 * (i & ~1),
+                make_float4(value(p, 0, s), value(p, 1, s), value(q, 0, s), value(q, 1, s)));
+        }
+    }
 }
 
 // ---- attention --------------------------------------------------------------------
@@ -280,6 +362,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
         }
     }
 
+    if (Src::kValues) __builtin_amdgcn_s_setprio(1);   // the other wave's products run under this one's softmax
     __builtin_amdgcn_sched_barrier(0);   // no loads of the next part early: they would cost registers
     // ---- softmax ----
     auto hidden = [&](int kg, int n, int e) { return 32 * kg + kv4::key_of(0, e) >= r.seen[n] - key0 - 4 * L; };
@@ -315,6 +398,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
         for (int t = 0; t < 2 * NB; ++t) r.o[n][t] *= corr;
     }
 
+    if (Src::kValues) __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     // ---- output ----
     if constexpr (Src::kValues && MODE != kApart) {
@@ -879,26 +963,50 @@ __global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict_
 
 }  // namespace
 
+// Blocks of a row that a workgroup takes: all of them at d_head 64 and 128.
+#define VH_KV4_BLOCKS(nb, LAUNCH) \
+    if ((nb) % 4 == 0) {          \
+        LAUNCH(4);                \
+    } else if ((nb) % 2 == 0) {   \
+        LAUNCH(2);                \
+    } else {                      \
+        LAUNCH(1);                \
+    }
+
 int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, const float* k, const float* v,
                       int T, int pos) {
-    VH_ARG(T >= 1 && n_kv >= 1 && d_head >= 32 && d_head % 32 == 0, "kv_append: bad shape");
+    VH_ARG(T >= 1 && n_kv >= 1 && n_kv <= 65535 && d_head >= 32 && d_head % 32 == 0, "kv_append: bad shape");
     VH_ARG(pos >= 0 && T <= max_seq - pos, "kv_append: %d rows at %d beyond max_seq %d", T, pos, max_seq);
-    const size_t n = 2 * (size_t)T * n_kv * (d_head / 32);
-    VH_LAUNCH(kv4_append_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, reinterpret_cast<uint8_t*>(L.k),
-              reinterpret_cast<uint8_t*>(L.v), reinterpret_cast<uint16_t*>(L.ks), reinterpret_cast<uint16_t*>(L.vs), k, v,
-              n_kv, d_head, max_seq, T, pos);
+    Kv4Append a;
+    a.k = k;
+    a.v = v;
+    a.kc = reinterpret_cast<uint8_t*>(L.k);
+    a.vc = reinterpret_cast<uint8_t*>(L.v);
+    a.ks = reinterpret_cast<uint16_t*>(L.ks);
+    a.vs = reinterpret_cast<uint16_t*>(L.vs);
+    a.ld = n_kv * d_head;
+    a.D = d_head;
+    a.max_seq = max_seq;
+    a.T = T;
+    a.pos = pos;
+    const int groups = (pos + T - 1) / kv4::kKeys - pos / kv4::kKeys + 1, nb = d_head / 32;
+#define VH_APPEND(CB) VH_LAUNCH(kv4_append_kernel<CB>, dim3(groups, n_kv, 2 * (nb / CB)), dim3(128 * CB), 0, s, a)
+    VH_KV4_BLOCKS(nb, VH_APPEND)
+#undef VH_APPEND
     VH_LAUNCHED();
     return VLRF_HIP_OK;
 }
 
 int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, int ctx_len, float* K,
                        float* V) {
-    VH_ARG(ctx_len >= 1 && ctx_len <= max_seq, "kv_dequant: ctx_len %d outside [0,%d]", ctx_len, max_seq);
-    const size_t n = (size_t)ctx_len * n_kv * (d_head / 2);
-    VH_LAUNCH(kv4_dequant_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
-              reinterpret_cast<const uint8_t*>(L.k), reinterpret_cast<const uint8_t*>(L.v),
-              reinterpret_cast<const uint16_t*>(L.ks), reinterpret_cast<const uint16_t*>(L.vs), n_kv, d_head, max_seq,
-              ctx_len, K, V);
+    VH_ARG(ctx_len >= 1 && ctx_len <= max_seq && n_kv <= 65535, "kv_dequant: ctx_len %d outside [0,%d]", ctx_len, max_seq);
+    const int groups = (ctx_len + kv4::kKeys - 1) / kv4::kKeys, nb = d_head / 32;
+#define VH_DEQUANT(CB)                                                                                              \
+    VH_LAUNCH(kv4_dequant_kernel<CB>, dim3(groups, n_kv, nb / CB), dim3(256), 0, s, reinterpret_cast<const uint8_t*>(L.k), \
+              reinterpret_cast<const uint8_t*>(L.v), reinterpret_cast<const uint16_t*>(L.ks),                       \
+              reinterpret_cast<const uint16_t*>(L.vs), n_kv * d_head, d_head, max_seq, ctx_len, K, V)
+    VH_KV4_BLOCKS(nb, VH_DEQUANT)
+#undef VH_DEQUANT
     VH_LAUNCHED();
     return VLRF_HIP_OK;
 }
