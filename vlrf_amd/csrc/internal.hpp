@@ -238,13 +238,23 @@ int launch_kv_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int
 // The 4-bit cache (kernels/kv4.hip): rows [pos, pos + T) quantized from k/v
 // [T][n_kv*d_head], rows [0, ctx_len) read back, and the attention of T query rows
 // [T][n_heads*d_head], the last T of ctx_len tokens (row t sees ctx_len - T + t + 1 keys).
+// The model's calls: rows of a wider buffer ([T][ld]), k and q rotated by the RoPE tables
+// as they are read, the position on the device (T 1; ctx_len is then the most there can
+// be), the result as bf16.
+struct Kv4Model {
+    const float* cos_t = nullptr;
+    const float* sin_t = nullptr;
+    int ld = 0;
+    const int* pos_dev = nullptr;
+    uint16_t* out16 = nullptr;
+};
 int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, const float* k, const float* v,
-                      int T, int pos);
+                      int T, int pos, const Kv4Model* m = nullptr);
 int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, int ctx_len, float* K,
                        float* V);
 // part: attn_kv4_part_bytes(...) bytes of device memory; ctr: a context's counters.
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
-                    int ctx_len, float scale, float* out, float* part, int* ctr);
+                    int ctx_len, float scale, float* out, float* part, int* ctr, const Kv4Model* m = nullptr);
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len);
 // Prefill: RoPE on k of T tokens of a [T][ld] QKV buffer at positions
 // pos0.., then the cache append of their K/V rows (q is left as it is: the

@@ -7,11 +7,11 @@
 // standing for (c - 8) * d: the encoder of vlrf_quantize_q4_0, bit for bit.  A
 // block that holds an infinity or a NaN gets a NaN scale and reads back as NaN.
 #include "../internal.hpp"
+#include "attn_core.hpp"
 #include "kv4_layout.hpp"
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 namespace vlrf_hip {
@@ -19,6 +19,9 @@ namespace {
 
 constexpr float kNegInf = -INFINITY;
 constexpr uint32_t kNanF16 = 0x7E00u;
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
 
 // f16(m / -8), the sign put on by hand: a block of zeros has -0, which the product
 // loses where the compiler fuses it into the conversion.
@@ -49,25 +52,46 @@ struct Kv4Append {
     uint8_t *kc, *vc;
     uint16_t *ks, *vs;
     int ld, D, max_seq, T, pos;
+    const int* pos_dev;       // the position, from the device (T 1); or null
+    const float *cos_t, *sin_t;   // [max_seq][D / 2] (ROPE)
 };
 
 __device__ __forceinline__ float quad_f(float v, int which) {   // the lane 1 or 2 away within its four
     return which == 1 ? dpp_f<0xB1>(v) : dpp_f<0x4E>(v);
 }
 
-template <int CB>
+// ROPE: K's rows are rotated at their positions first (rope.hpp:75-99), the element half a
+// head away read beside the own one.
+template <int CB, bool ROPE>
 __global__ __launch_bounds__(128 * CB) void kv4_append_kernel(Kv4Append a) {
     __shared__ uint32_t codes[128 * CB];
     __shared__ uint16_t scales[32 * CB];
     const int tid = threadIdx.x, bl = tid % (4 * CB) / 4, word = tid % 4, slot_key = tid / (4 * CB);
     const bool isv = blockIdx.z & 1;
     const int nb = a.D / 32, b = (int)(blockIdx.z >> 1) * CB + bl, g = blockIdx.y;
-    const int kb = a.pos / kv4::kKeys + (int)blockIdx.x, t = kb * kv4::kKeys + slot_key, row = t - a.pos;
+    const int pos = a.pos_dev ? *a.pos_dev : a.pos;
+    if (pos < 0 || pos > a.max_seq - a.T) return;   // host checks capacity; never write past the cache
+    const int kb = pos / kv4::kKeys + (int)blockIdx.x, t = kb * kv4::kKeys + slot_key, row = t - pos;
     const bool on = row >= 0 && row < a.T;
-    const bool whole = kb * kv4::kKeys >= a.pos && (kb + 1) * kv4::kKeys <= a.pos + a.T;
+    const bool whole = kb * kv4::kKeys >= pos && (kb + 1) * kv4::kKeys <= pos + a.T;
 
     float e[8] = {};
-    if (on) __builtin_memcpy(e, (isv ? a.v : a.k) + (size_t)row * a.ld + g * a.D + 32 * b + 8 * word, 32);
+    const float* from = (isv ? a.v : a.k) + (size_t)row * a.ld + g * a.D;
+    const int el = 32 * b + 8 * word;
+    if (on) __builtin_memcpy(e, from + el, 32);
+    if (ROPE && on && !isv) {
+        const int half = a.D / 2, j = el < half ? el : el - half;   // half is a multiple of 8
+        float o[8], cr[8], sr[8];
+        __builtin_memcpy(o, from + (el < half ? el + half : j), 32);
+        __builtin_memcpy(cr, a.cos_t + (size_t)t * half + j, 32);
+        __builtin_memcpy(sr, a.sin_t + (size_t)t * half + j, 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float y0, y1;
+            attn::rope2(el < half ? e[i] : o[i], el < half ? o[i] : e[i], cr[i], sr[i], &y0, &y1);
+            e[i] = el < half ? y0 : y1;
+        }
+    }
     // The largest magnitude, the first of equal ones: the maximum of (|x|, -index, sign).
     float amax = 0.f, m = 0.f;
     bool bad = false;
@@ -131,8 +155,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
                                                           int ctx, float* __restrict__ K, float* __restrict__ V) {
     const int nb = D / 32, b0 = blockIdx.z * CB, g = blockIdx.y, t0 = blockIdx.x * kv4::kKeys, tid = threadIdx.x;
     const size_t cb = g * kv4::head_codes(max_seq, D), sb = g * kv4::head_scales(max_seq, D);
+    // Past the caches (nontemporal): what is written here is far more than they hold, or
+    // read once (30001 rows of 8B shape 69.0 -> 58.6 us, 4096 of 1.1B shape 4.8 -> 4.4).
     auto put = [&](float* to, int t, int e, float4 x) {
-        if (t < ctx) __builtin_memcpy(to + (size_t)t * row + g * D + e, &x, 16);
+        if (t < ctx) __builtin_nontemporal_store(__builtin_bit_cast(f4v, x), reinterpret_cast<f4v*>(to + (size_t)t * row + g * D + e));
     };
     auto value = [](uint32_t w, int i, float d) { return (float)((int)(w >> (4 * i) & 15u) - 8) * d; };
     constexpr int KI = 256 * CB;   // items of K: 32 keys, 8 CB times four elements
@@ -167,8 +193,14 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 
 // ---- attention --------------------------------------------------------------------
 // The T * rep query rows of a KV head (rep query heads share it) stand as rows t rep
-// + r, 16 NG of them a workgroup; its four waves take the chunk's groups of 32 keys
-// in turn, each with its own running maximum and sum, and merge through LDS.
+// + r.  For few of them a workgroup takes 16, and where blocks of 16 are few several
+// share a block's keys: the eight waves of each take groups of 32 keys in turn, each
+// with its own running maximum and sum, and merge through LDS, and the workgroup that
+// comes last merges all of a block's.
+// One decode row at 32/8 heads of 128: 120001 keys 42 us (138 MB, 3.3 TB/s with the
+// launch, its first loads and the merge: 4.0 TB/s without, what a large read reaches),
+// 15001 keys 12 (17 MB: 1.4 TB/s; bound by that chain of waits, two groups a wave); 4096
+// keys at 32/4 heads of 64 8 us.
 //   scores   S^T = K Q^T, 16 keys by 16 rows and a block of 32 elements an
 //            instruction.  A code minus 8 is exact in f16; q, scaled by a power of
 //            two for the row's largest element to lie in [2^13, 2^14), enters as two
@@ -182,22 +214,21 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // A lane's scores are of the row that is its column in both products and of the keys
 // that its group of V's layout holds, so nothing moves between lanes but the
 // maximum's two exchanges a group.
-typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef float f4v __attribute__((ext_vector_type(4)));
-
 constexpr float kHeadroom = 4.f, kWeightBits = 10.f;
 
 struct Kv4Attn {
-    const float* q;          // [T][n_heads][D]
+    const float* q;          // [T][ldq], n_heads * D of a row
     const uint8_t *kc, *vc;  // the layer's codes and scales
     const uint16_t *ks, *vs;
-    float *out, *part;       // [T][n_heads][D]; [T][n_heads][nch][D + 2] where nch > 1
+    float *out, *part;       // [T][n_heads][D]; [T][n_heads][nch][kv4_part(D)] where nch > 1
     int* ctr;                // a counter a block, zero between launches: the merge in this launch; or null
     size_t codes, scales;    // of a head
-    int n_heads, rep, T, ctx;
+    uint16_t* out16;         // the result as bf16 instead of out; or null
+    const int* pos_dev;      // T 1: ctx is one more than this (at most ctx); or null
+    const float *cos_t, *sin_t;   // [max_seq][D / 2]: q is rotated at its position as it is read; or null
+    int n_heads, rep, T, ctx, ldq;
     uint32_t magic;          // floor(2^32 / rep) + 1: row / rep is the high word of row * magic while row * rep < 2^32
-    int rounds, nch;         // groups of 32 keys a wave takes, chunks of the context
+    int nch;                 // workgroups that share the keys of a block of rows
     float sl2, qsign;        // |scale| log2(e), the scale's sign
 };
 
@@ -205,10 +236,20 @@ __device__ __forceinline__ int kv4_token(const Kv4Attn& a, int row) {
     return a.rep == 1 ? row : (int)__umulhi((uint32_t)row, a.magic);
 }
 
-// Row `row` of KV head g among the T * n_heads rows of q.
-__device__ __forceinline__ size_t kv4_q_row(const Kv4Attn& a, int g, int row) {
+// Row `row` of KV head g among the T * n_heads rows of the result.
+__device__ __forceinline__ size_t kv4_row(const Kv4Attn& a, int g, int row) {
     const int t = kv4_token(a, row);
     return (size_t)t * a.n_heads + g * a.rep + (row - t * a.rep);
+}
+
+// Four elements of the result from element i on.
+__device__ __forceinline__ void kv4_store(float* out, uint16_t* out16, size_t i, const float (&x)[4]) {
+    if (out16) {
+        const uint2 y = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        __builtin_memcpy(out16 + i, &y, 8);
+    } else {
+        __builtin_memcpy(out + i, x, 16);
+    }
 }
 
 __device__ __forceinline__ h2v as_h2(uint32_t u) { return __builtin_bit_cast(h2v, u); }
@@ -285,16 +326,27 @@ __device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn&
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
         const int row = min(row0 + 16 * n + c, R - 1);   // rows past the last one repeat it and are not stored
-        const float* qp = a.q + kv4_q_row(a, g, row) * (32 * NB) + 8 * L;
-        float x[NB][8], amax = 0.f;
+        const int t = kv4_token(a, row), at = a.ctx - a.T + t;
+        const float* qp = a.q + (size_t)t * a.ldq + (g * a.rep + (row - t * a.rep)) * (32 * NB) + 8 * L;
+        float y[NB][8], x[NB][8], amax = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) __builtin_memcpy(y[b], qp + 32 * b, 32);
+        if (a.cos_t) {   // a pair's elements are half a head apart: both are the lane's
+#pragma unroll
+            for (int b = 0; b < NB / 2; ++b) {
+                float cr[8], sr[8];
+                __builtin_memcpy(cr, a.cos_t + (size_t)at * (16 * NB) + 32 * b + 8 * L, 32);
+                __builtin_memcpy(sr, a.sin_t + (size_t)at * (16 * NB) + 32 * b + 8 * L, 32);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) attn::rope2(y[b][e], y[b + NB / 2][e], cr[e], sr[e], &y[b][e], &y[b + NB / 2][e]);
+            }
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float y[8];
-            __builtin_memcpy(y, qp + 32 * b, 32);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[e];   // in the order of codes8
+            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[b][e];   // in the order of codes8
 #pragma unroll
-            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[b][e]));
         }
         amax = over_groups_max(amax);
         const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 60);
@@ -308,11 +360,11 @@ __device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn&
             r.qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
             r.ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
         }
-        r.seen[n] = a.ctx - a.T + 1 + kv4_token(a, row);
+        r.seen[n] = at + 1;
         r.m2[n] = kNegInf;
         r.l[n] = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2 * NB; ++t) r.o[n][t] = f4v{};
+        for (int i = 0; i < 2 * NB; ++i) r.o[n][i] = f4v{};
     }
 }
 
@@ -580,7 +632,8 @@ struct Kv4MergeLds {
 };
 
 template <int D, bool COHERENT, class At>
-__device__ __forceinline__ void kv4_merge(Kv4MergeLds<D>& sm, const float* part, int nch, int rows, float* out, At row_at) {
+__device__ __forceinline__ void kv4_merge(Kv4MergeLds<D>& sm, const float* part, int nch, int rows, float* out,
+                                          uint16_t* out16, At row_at) {
     constexpr int B = 8, Q = D / 4, PS = kv4_part(D), AUX = COHERENT ? 16 : 0;   // 16: sc1, past this die's L2
     const int n = rows * Q, P = 512 / n, tid = threadIdx.x, share = tid / n, i = tid - share * n;
     const bool on = share < P;
@@ -636,7 +689,7 @@ __device__ __forceinline__ void kv4_merge(Kv4MergeLds<D>& sm, const float* part,
     if (!on || share) return;
     const float by = sum == 0.f ? 0.f : 1.f / sum;
     const float x[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
-    __builtin_memcpy(out + at * D + 4 * (i % Q), x, 16);
+    kv4_store(out, out16, at * D + 4 * (i % Q), x);
 }
 
 constexpr int kWaves = 8;   // of a workgroup of 16 rows
@@ -655,13 +708,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
         Kv4MergeLds<D> merge;
     } lds;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
+    if (a.pos_dev) a.ctx = min(*a.pos_dev + 1, a.ctx);
     const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, row0 = blockIdx.z * ROWS, R = a.T * a.rep;
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
     const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
     // Keys that the block's first and last row see.
     const int past = a.ctx - a.T + 1, fewest = past + kv4_token(a, row0), most = past + kv4_token(a, min(row0 + ROWS - 1, R - 1));
-    const int kb0 = chunk * kWaves * a.rounds + w;
-    const int mine = min(a.rounds, max(0, ((most + kv4::kKeys - 1) / kv4::kKeys - kb0 + kWaves - 1) / kWaves));
+    // The wave's groups of keys: every nch * kWaves-th, so that all share any context alike.
+    const int kb0 = chunk * kWaves + w, stride = nch * kWaves;
+    auto mine_of = [&](int groups) { return groups > kb0 ? (groups - kb0 + stride - 1) / stride : 0; };
+    const int mine = mine_of((most + kv4::kKeys - 1) / kv4::kKeys), inside = min(mine, mine_of(fewest / kv4::kKeys));
 
     Kv4Raw<NB> raw;
     raw.magic = magic1024();
@@ -671,7 +727,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     // Three loops of one body each (two in one would cost each other registers): the groups
     // that every row sees whole, those at some row's edge, and those of both that the first
     // two left because of a large scale.
-    const int inside = max(0, min(mine, (fewest / kv4::kKeys - kb0 + kWaves - 1) / kWaves));
     bool left = false;
     auto large = [&](const Kv4Raw<NB>& x) {   // a scale of 2 or more, or no number
         uint32_t any = 0;
@@ -679,24 +734,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
         for (int b = 0; b < NB; ++b) any |= x.vd[b].x | x.vd[b].y | x.vd[b].z | x.vd[b].w;
         return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
     };
-    auto load = [&](int i) { kv4_load<NB>(raw, kc, vc, ks, vs, kb0 + i * kWaves, c, L); };   // i < mine
+    auto load = [&](int i) { kv4_load<NB>(raw, kc, vc, ks, vs, kb0 + i * stride, c, L); };   // i < mine
     int i = 0;
     for (; i < inside; ++i) {
         const Kv4Raw<NB> cur = raw;
         if (i + 1 < mine) load(i + 1);
         if (large(cur)) left = true;
-        else kv4_keys<kInside, 1>(r, cur, (kb0 + i * kWaves) * kv4::kKeys, L);
+        else kv4_keys<kInside, 1>(r, cur, (kb0 + i * stride) * kv4::kKeys, L);
     }
     for (; i < mine; ++i) {
         const Kv4Raw<NB> cur = raw;
         if (i + 1 < mine) load(i + 1);
         if (large(cur)) left = true;
-        else kv4_keys<kEdge, 1>(r, cur, (kb0 + i * kWaves) * kv4::kKeys, L);
+        else kv4_keys<kEdge, 1>(r, cur, (kb0 + i * stride) * kv4::kKeys, L);
     }
     if (left)
         for (i = 0; i < mine; ++i) {
             load(i);
-            if (large(raw)) kv4_keys<kApart, 1>(r, raw, (kb0 + i * kWaves) * kv4::kKeys, L);
+            if (large(raw)) kv4_keys<kApart, 1>(r, raw, (kb0 + i * stride) * kv4::kKeys, L);
         }
 
     // ---- the waves' results, then the chunk's ----
@@ -733,12 +788,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
             l = fmaf(f, x.l[k][j], l);
             v[0] = fmaf(f, y.x, v[0]); v[1] = fmaf(f, y.y, v[1]); v[2] = fmaf(f, y.z, v[2]); v[3] = fmaf(f, y.w, v[3]);
         }
-        const size_t at = kv4_q_row(a, g, row0 + j);
+        const size_t at = kv4_row(a, g, row0 + j);
         if (nch == 1) {
             const float by = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] *= by;
-            __builtin_memcpy(a.out + at * D + e, v, 16);
+            kv4_store(a.out, a.out16, at * D + e, v);
             continue;
         }
         // Past this die's L2 (sc1): read by another workgroup of this launch.
@@ -759,7 +814,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     }
     __syncthreads();
     if (!last) return;
-    kv4_merge<D, true>(lds.merge, a.part, nch, rows, a.out, [&](int j) { return kv4_q_row(a, g, row0 + j); });
+    kv4_merge<D, true>(lds.merge, a.part, nch, rows, a.out, a.out16, [&](int j) { return kv4_row(a, g, row0 + j); });
 }
 
 // ---- many rows --------------------------------------------------------------------
@@ -941,7 +996,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         const float sum = over_groups_sum(r.l[n]);
         const int row = row0 + 16 * n + c;
         if (row >= R) continue;
-        const size_t at = kv4_q_row(a, g, row);
+        const size_t at = kv4_row(a, g, row);
         const float by = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -949,16 +1004,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
             for (int h = 0; h < 2; ++h) {
                 const float x[4] = {r.o[n][2 * b][2 * h] * by, r.o[n][2 * b + 1][2 * h] * by, r.o[n][2 * b][2 * h + 1] * by,
                                     r.o[n][2 * b + 1][2 * h + 1] * by};
-                __builtin_memcpy(a.out + at * D + 32 * b + 8 * L + 4 * h, x, 16);
+                kv4_store(a.out, a.out16, at * D + 32 * b + 8 * L + 4 * h, x);
             }
     }
 }
 
 // The merge as a launch of its own: a row a workgroup.
 template <int D>
-__global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, float* __restrict__ out) {
+__global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, float* __restrict__ out,
+                                                        uint16_t* __restrict__ out16) {
     __shared__ Kv4MergeLds<D> sm;
-    kv4_merge<D, false>(sm, part, nch, 1, out, [](int) { return (size_t)blockIdx.x; });
+    kv4_merge<D, false>(sm, part, nch, 1, out, out16, [](int) { return (size_t)blockIdx.x; });
 }
 
 }  // namespace
@@ -974,9 +1030,10 @@ __global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict_
     }
 
 int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int max_seq, const float* k, const float* v,
-                      int T, int pos) {
+                      int T, int pos, const Kv4Model* m) {
     VH_ARG(T >= 1 && n_kv >= 1 && n_kv <= 65535 && d_head >= 32 && d_head % 32 == 0, "kv_append: bad shape");
     VH_ARG(pos >= 0 && T <= max_seq - pos, "kv_append: %d rows at %d beyond max_seq %d", T, pos, max_seq);
+    VH_ARG(!m || (m->cos_t && m->sin_t && m->ld >= n_kv * d_head && (!m->pos_dev || T == 1)), "kv_append: bad model call");
     Kv4Append a;
     a.k = k;
     a.v = v;
@@ -984,14 +1041,24 @@ int launch_kv4_append(hipStream_t s, const KVLayer& L, int n_kv, int d_head, int
     a.vc = reinterpret_cast<uint8_t*>(L.v);
     a.ks = reinterpret_cast<uint16_t*>(L.ks);
     a.vs = reinterpret_cast<uint16_t*>(L.vs);
-    a.ld = n_kv * d_head;
+    a.ld = m ? m->ld : n_kv * d_head;
+    a.pos_dev = m ? m->pos_dev : nullptr;
+    a.cos_t = m ? m->cos_t : nullptr;
+    a.sin_t = m ? m->sin_t : nullptr;
     a.D = d_head;
     a.max_seq = max_seq;
     a.T = T;
     a.pos = pos;
     const int groups = (pos + T - 1) / kv4::kKeys - pos / kv4::kKeys + 1, nb = d_head / 32;
-#define VH_APPEND(CB) VH_LAUNCH(kv4_append_kernel<CB>, dim3(groups, n_kv, 2 * (nb / CB)), dim3(128 * CB), 0, s, a)
-    VH_KV4_BLOCKS(nb, VH_APPEND)
+#define VH_APPEND(CB, R) VH_LAUNCH((kv4_append_kernel<CB, R>), dim3(groups, n_kv, 2 * (nb / CB)), dim3(128 * CB), 0, s, a)
+#define VH_APPEND_AS(CB) VH_APPEND(CB, false)
+    if (m) {   // d_head 64 or 128
+        if (nb == 4) VH_APPEND(4, true);
+        else VH_APPEND(2, true);
+    } else {
+        VH_KV4_BLOCKS(nb, VH_APPEND_AS)
+    }
+#undef VH_APPEND_AS
 #undef VH_APPEND
     VH_LAUNCHED();
     return VLRF_HIP_OK;
@@ -1014,23 +1081,38 @@ int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, in
 namespace {
 struct Kv4Plan {
     bool tiles = false;                      // the kernel for many rows
-    int blocks = 1, rounds = 1, nch = 1;     // blocks of rows of a KV head
+    int blocks = 1, nch = 1;                 // blocks of rows of a KV head, workgroups that share a block's keys
 };
+
+// The kernel for many rows wins once its workgroups fill the CUs (rows kernel's / tiles kernel's
+// time): 1777 rows of 4001 keys at 32/8 heads of 128 (448 workgroups) 406 / 228 us, 1024 of 1024
+// (256) 76 / 60, 1024 of 2048 at 32/4 of 64 (256) 64 / 63; but 700 of 4000 (176) 197 / 206, 512 of
+// 1024 (128) 46 / 57.  Below, blocks of 16 rows, whose keys are shared out to as many
+// workgroups as there are CUs, one group of keys or more for each wave.  One decode row at
+// 32/8 heads of 128 with 128, 256, 384 and 512 workgroups in all: 15001 keys 15.7, 12.5, 18.3, 16.8 us;
+// 120001 keys 64, 42, 52, 47 (two of them stand on a CU, but 384 leave half with one).
+constexpr long kTilesFrom = 240, kSharers = 256;
 
 Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
     Kv4Plan p;
     const long R = (long)T * (n_heads / n_kv);
     p.blocks = (int)((R + kTileRows - 1) / kTileRows);
-    if ((long)p.blocks * n_kv >= (std::getenv("KV4_TILES") ? atol(std::getenv("KV4_TILES")) : 240)) {
+    if ((long)p.blocks * n_kv >= kTilesFrom) {
         p.tiles = true;
         return p;
     }
     p.blocks = (int)((R + 15) / 16);
-    const long nb = (ctx_len + kv4::kKeys - 1) / kv4::kKeys, want = std::getenv("KV4_WANT") ? atol(std::getenv("KV4_WANT")) : 2048;
-    p.rounds = (int)((nb * p.blocks * n_kv + want - 1) / want);
-    p.nch = (int)((nb + kWaves * p.rounds - 1) / (kWaves * p.rounds));
+    const long groups = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
+    p.nch = (int)std::max(1l, std::min((groups + kWaves - 1) / kWaves, kSharers / ((long)p.blocks * n_kv)));
     return p;
 }
+
+// The last workgroup of a block merges its chunks, up to 32 of them; more are merged by a launch
+// of their own, a workgroup a row.  In the launch / in one of its own, us: 16 chunks (32/4 heads of 64, 4096
+// keys) 8.1 / 9.4, 32 (32/8 of 128, 15001) 12.5 / 13.3, 59 (8/1 of 128, 15001) 12.9 / 10.3, 235 (60001)
+// 26.5 / 11.9.
+constexpr int kMergedChunks = 32;
+static_assert(kSharers <= kSmallMaxTiles, "a counter for each block whose keys are shared");
 }  // namespace
 
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
@@ -1040,12 +1122,13 @@ size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len
 }
 
 int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads, int n_kv, int d_head, int max_seq, int T,
-                    int ctx_len, float scale, float* out, float* part, int* ctr) {
+                    int ctx_len, float scale, float* out, float* part, int* ctr, const Kv4Model* m) {
     VH_ARG(n_kv >= 1 && n_heads >= 1 && n_heads % n_kv == 0, "attn: n_heads %d not a multiple of n_kv %d", n_heads, n_kv);
     VH_ARG(d_head == 64 || d_head == 128, "attn: d_head %d not in {64,128}", d_head);
     VH_ARG(ctx_len >= 1 && ctx_len <= max_seq && T >= 1 && T <= ctx_len, "attn: %d rows of %d keys in a cache of %d", T,
            ctx_len, max_seq);
     VH_ARG((long)T * n_heads < (1l << 31), "attn: %d rows of %d heads", T, n_heads);
+    VH_ARG(!m || (m->ld >= n_heads * d_head && (!m->pos_dev || T == 1)), "attn: bad model call");
     const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
     VH_ARG(p.blocks <= 65535 && n_kv <= 65535 && (size_t)T * n_heads / n_kv * (n_heads / n_kv) < (1ull << 32),
            "attn: %d rows of %d heads over %d KV heads are beyond a launch", T, n_heads, n_kv);
@@ -1058,7 +1141,7 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     a.vs = reinterpret_cast<const uint16_t*>(L.vs);
     a.out = out;
     a.part = part;
-    const bool merged = ctr && (long)p.blocks * n_kv <= kSmallMaxTiles && p.nch <= (std::getenv("KV4_M") ? atoi(std::getenv("KV4_M")) : 32);
+    const bool merged = ctr && p.nch <= kMergedChunks;
     a.ctr = merged ? ctr : nullptr;
     a.codes = kv4::head_codes(max_seq, d_head);
     a.scales = kv4::head_scales(max_seq, d_head);
@@ -1067,7 +1150,11 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     a.magic = (uint32_t)((1ull << 32) / a.rep + 1);
     a.T = T;
     a.ctx = ctx_len;
-    a.rounds = p.rounds;
+    a.ldq = m ? m->ld : n_heads * d_head;
+    a.out16 = m ? m->out16 : nullptr;
+    a.pos_dev = m ? m->pos_dev : nullptr;
+    a.cos_t = m ? m->cos_t : nullptr;
+    a.sin_t = m ? m->sin_t : nullptr;
     a.nch = p.nch;
     // Never 0: a masked score's -inf times the factor has to stay -inf.
     a.sl2 = std::max((float)(std::fabs((double)scale) * 1.4426950408889634), 1e-20f);
@@ -1084,8 +1171,8 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
     else VH_LAUNCH(kv4_attn_rows_kernel<128>, grid, dim3(64 * kWaves), 0, s, a);
     VH_LAUNCHED();
     if (p.nch == 1 || merged) return VLRF_HIP_OK;
-    if (d_head == 64) VH_LAUNCH(kv4_merge_kernel<64>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out);
-    else VH_LAUNCH(kv4_merge_kernel<128>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out);
+    if (d_head == 64) VH_LAUNCH(kv4_merge_kernel<64>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out, a.out16);
+    else VH_LAUNCH(kv4_merge_kernel<128>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out, a.out16);
     VH_LAUNCHED();
     return VLRF_HIP_OK;
 }

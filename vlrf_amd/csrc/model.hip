@@ -171,7 +171,16 @@ int enqueue_step(vlrf_hip_model* m, hipStream_t s) {
                     rc = launch_qlinear(s, Ly.wqkv, m->x, m->qkv, 1, Ly.ln1, eps, nullptr);
             }
             lk(VLRF_HIP_LK_ATTN);
-            if (!rc) rc = launch_attn_decode(s, q, Ly.kv.k, Ly.kv.v, Ly.kv.ks, Ly.kv.vs, Ly.kv.dtype,
+            if (!rc && Ly.kv.dtype == VLRF_HIP_KV_Q4_0) {   // k and q are rotated as they are read
+                Kv4Model k4;
+                k4.cos_t = m->cos_t;
+                k4.sin_t = m->sin_t;
+                k4.ld = m->D + 2 * m->dkv;
+                k4.pos_dev = m->state + 1;
+                rc = launch_kv4_append(s, Ly.kv, m->G, m->dh, m->S, k, v, 1, 0, &k4);
+                if (!rc) rc = launch_attn_kv4(s, q, Ly.kv, m->H, m->G, m->dh, m->S, 1, m->S, scale, m->att, m->part,
+                                              m->ctx->small_tile_ctr, &k4);
+            } else if (!rc) rc = launch_attn_decode(s, q, Ly.kv.k, Ly.kv.v, Ly.kv.ks, Ly.kv.vs, Ly.kv.dtype,
                                              (long)m->S * m->dh, m->H, m->G, m->dh, 1, m->state + 1,
                                              m->n_splits, scale, m->part, m->att, &fz);
         }
@@ -318,8 +327,10 @@ int vlrf_hip_model_create(vlrf_hip_ctx_t ctx, const vlrf_hip_model_config* cfg, 
     VH_ARG(c.d_model % 32 == 0 && c.d_ff % 32 == 0, "model: d_model and d_ff must be multiples of 32");
     VH_ARG(c.weight_dtype == VLRF_HIP_DT_Q8_0 || c.weight_dtype == VLRF_HIP_DT_Q4_0 || c.weight_dtype == VLRF_HIP_DT_F32,
            "model: unsupported weight dtype %d", c.weight_dtype);
-    VH_ARG(c.kv_dtype == VLRF_HIP_KV_F32 || c.kv_dtype == VLRF_HIP_KV_F16 || c.kv_dtype == VLRF_HIP_KV_Q8_0,
+    VH_ARG(c.kv_dtype == VLRF_HIP_KV_F32 || c.kv_dtype == VLRF_HIP_KV_F16 || c.kv_dtype == VLRF_HIP_KV_Q8_0 ||
+               c.kv_dtype == VLRF_HIP_KV_Q4_0,
            "model: unsupported KV cache dtype %d", c.kv_dtype);
+    const bool kv4 = c.kv_dtype == VLRF_HIP_KV_Q4_0;   // its own append and attention, no fused or chunked form
 
     auto* m = new (std::nothrow) vlrf_hip_model();
     if (!m) return VLRF_HIP_ERR_NOMEM;
@@ -347,9 +358,10 @@ int vlrf_hip_model_create(vlrf_hip_ctx_t ctx, const vlrf_hip_model_config* cfg, 
     dalloc((void**)&m->h, (size_t)m->F * 4);
     dalloc((void**)&m->logits, (size_t)m->V * 4);
     dalloc((void**)&m->argpairs, 512 * sizeof(float2));
-    dalloc((void**)&m->part, (size_t)m->H * m->n_splits * (dh + 2) * 4);
+    dalloc((void**)&m->part, std::max((size_t)m->H * m->n_splits * (dh + 2) * 4,
+                                      kv4 ? attn_kv4_part_bytes(m->H, m->G, dh, 1, m->S) : 0));
     // Chunked decode attention when the O projection's GEMV can merge it.
-    m->nch = c.weight_dtype == VLRF_HIP_DT_Q8_0 || c.weight_dtype == VLRF_HIP_DT_Q4_0
+    m->nch = !kv4 && (c.weight_dtype == VLRF_HIP_DT_Q8_0 || c.weight_dtype == VLRF_HIP_DT_Q4_0)
                  ? attn_decode_chunks(m->S, dh, m->G) : 0;
     DevWeight wo_shape;
     wo_shape.dtype = c.weight_dtype;
@@ -361,7 +373,7 @@ int vlrf_hip_model_create(vlrf_hip_ctx_t ctx, const vlrf_hip_model_config* cfg, 
     // Q8_0/F16 caches (an F32 cache's rounds need more registers than the
     // fused kernel keeps: it would spill).
     const char* qa_env = std::getenv("VLRF_HIP_QKV_ATTN");
-    if (!(qa_env && std::strcmp(qa_env, "0") == 0) && c.kv_dtype != VLRF_HIP_KV_F32 && dh == 64 && m->G <= 8 &&
+    if (!(qa_env && std::strcmp(qa_env, "0") == 0) && c.kv_dtype != VLRF_HIP_KV_F32 && !kv4 && dh == 64 && m->G <= 8 &&
         wo_shape.K == m->D) {
         const int n = (m->S + kAttnChunkRows - 1) / kAttnChunkRows;
         if (n + 1 <= qlinear_merge_max_chunks(wo_shape) &&
@@ -416,8 +428,8 @@ int vlrf_hip_model_create(vlrf_hip_ctx_t ctx, const vlrf_hip_model_config* cfg, 
     // Every layer's K, V and row scales in one allocation (each on its own 256
     // bytes), so that a reset clears them in one go.
     auto up256 = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    const size_t kvdata = up256((size_t)m->G * m->S * dh * kv_elem_bytes(c.kv_dtype));
-    const size_t kvscales = c.kv_dtype == VLRF_HIP_KV_Q8_0 ? up256((size_t)m->S * 4) : 0;
+    const size_t kvdata = up256(kv_data_bytes(c.kv_dtype, m->G, m->S, dh));
+    const size_t kvscales = up256(kv_scale_bytes(c.kv_dtype, m->G, m->S, dh));
     m->kv_bytes = 2 * (kvdata + kvscales) * m->L;
     dalloc((void**)&m->kv_all, m->kv_bytes);
     int8_t* kv_at = m->kv_all;
@@ -637,7 +649,8 @@ int prefill_reserve(vlrf_hip_model* m, int T) {
     size_t need = 0;
     if (!m->layers.empty()) {
         const Layer& L0 = m->layers[0];
-        need = std::max({qgemm_part_bytes(L0.wqkv, T, false), qgemm_part_bytes(L0.wo, T, false),
+        if (m->cfg.kv_dtype == VLRF_HIP_KV_Q4_0) need = attn_kv4_part_bytes(m->H, m->G, m->dh, T, m->pos + T);
+        need = std::max({need, qgemm_part_bytes(L0.wqkv, T, false), qgemm_part_bytes(L0.wo, T, false),
                          qgemm_part_bytes(L0.wg, T, true), qgemm_part_bytes(L0.wd, T, false)});
     }
     if (need > m->pf_part_bytes) {
@@ -695,9 +708,20 @@ int enqueue_prefill_layers(vlrf_hip_model* m, const float* x_in, float* x_out, i
         rc = launch_rows_to_bf16(s, src, Ly.ln1, m->pf_a, T, m->D, eps);
         if (!rc) rc = launch_qgemm(s, Ly.wqkv, m->pf_a, T, nullptr, m->pf_qkv, m->pf_part);
         // k rotated and appended here; q rotated by the attention as it loads it
-        if (!rc) rc = launch_prefill_rope_append(s, Ly.kv, m->pf_qkv, ld, T, m->H, m->G, m->dh, m->S, m->pos,
+        if (!rc && Ly.kv.dtype == VLRF_HIP_KV_Q4_0) {
+            Kv4Model k4;
+            k4.cos_t = m->cos_t;
+            k4.sin_t = m->sin_t;
+            k4.ld = ld;
+            k4.out16 = m->pf_att;
+            const float* k = m->pf_qkv + m->D;
+            rc = launch_kv4_append(s, Ly.kv, m->G, m->dh, m->S, k, k + m->dkv, T, m->pos, &k4);
+            if (!rc) rc = launch_attn_kv4(s, m->pf_qkv, Ly.kv, m->H, m->G, m->dh, m->S, T, m->pos + T, scale, nullptr,
+                                          m->pf_part, m->ctx->small_tile_ctr, &k4);
+        } else if (!rc) rc = launch_prefill_rope_append(s, Ly.kv, m->pf_qkv, ld, T, m->H, m->G, m->dh, m->S, m->pos,
                                                  m->cos_t, m->sin_t);
-        if (!rc) rc = launch_attn_prefill(s, m->pf_qkv, ld, Ly.kv, T, m->pos, m->H, m->G, m->dh, m->S, scale,
+        if (!rc && Ly.kv.dtype != VLRF_HIP_KV_Q4_0)
+            rc = launch_attn_prefill(s, m->pf_qkv, ld, Ly.kv, T, m->pos, m->H, m->G, m->dh, m->S, scale,
                                           m->cos_t, m->sin_t, m->pf_att);
         if (!rc) rc = launch_qgemm(s, Ly.wo, m->pf_att, T, src, x, m->pf_part);   // x = src + att . Wo^T
         if (!rc) rc = launch_rows_to_bf16(s, x, Ly.ln2, m->pf_a, T, m->D, eps);
@@ -894,8 +918,8 @@ int vlrf_hip_model_step_bytes(vlrf_hip_model_t m, int ctx_len, double out[3]) {
     w += (double)weight_device_bytes(m->lm_head.dtype, m->V, m->D);
     // K and V elements of the context (plus one f32 scale per row for Q8_0), per layer.
     const bool q8 = m->cfg.kv_dtype == VLRF_HIP_KV_Q8_0;
-    const double kv = (double)m->L * (2.0 * ctx_len * m->dkv * kv_elem_bytes(m->cfg.kv_dtype) +
-                                      (q8 ? 2.0 * ctx_len * 4.0 : 0.0));
+    const double element = m->cfg.kv_dtype == VLRF_HIP_KV_Q4_0 ? 18.0 / 32.0 : kv_elem_bytes(m->cfg.kv_dtype);
+    const double kv = (double)m->L * (2.0 * ctx_len * m->dkv * element + (q8 ? 2.0 * ctx_len * 4.0 : 0.0));
     // Norm weights (2 per layer + final) and the embedding row.
     const double other = (2.0 * m->L + 1.0) * m->D * 4.0 + m->D * 4.0;
     out[0] = w;

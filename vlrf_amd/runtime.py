@@ -299,10 +299,15 @@ class Model:
 
     def kv_rows(self, layer, row0, n):
         """(K [n,row], V, K scales [n], V scales) of the model's cache: int8 codes
-        and f32 scales (Q8_0), or uint16 f16 bits / float32 with scales None."""
+        and f32 scales (Q8_0), or uint16 f16 bits / float32 with scales None; KV_Q4_0:
+        uint8 [n, row/32, 18] blocks."""
         c = self.cfg
         row = c["n_kv_heads"] * (c["d_model"] // c["n_heads"])
         dt = c.get("kv_dtype", KV_Q8_0)
+        if dt == KV_Q4_0:
+            kb, vb = (np.zeros((n, row // 32, 18), np.uint8) for _ in range(2))
+            check(lib().vlrf_hip_model_kv_read(self.h, layer, row0, n, kb.ctypes.data, vb.ctypes.data, None, None))
+            return kb, vb, None, None
         et = {KV_F32: np.float32, KV_F16: np.uint16}.get(dt, np.int8)
         kq, vq = np.zeros((n, row), et), np.zeros((n, row), et)
         q8 = dt == KV_Q8_0
