@@ -280,10 +280,14 @@ __device__ __forceinline__ h8v h8_of(h2v a, h2v b, h2v c, h2v d) { return h8v{a.
 // multiplied: the compiler would form it twice, by a conversion of the rounded
 // product and by one that is fused with the product, which now and then differ.
 __device__ __forceinline__ void split2(float x, float f, float y, float g, h2v& hi, h2v& lo) {
-    uint32_t h = __builtin_bit_cast(uint32_t, h2v{(_Float16)fmaf(x, f, 0.f), (_Float16)fmaf(y, g, 0.f)});
+    float u = fmaf(x, f, 0.f), v = fmaf(y, g, 0.f);
+    asm("" : "+v"(u), "+v"(v));
+    uint32_t h = __builtin_bit_cast(uint32_t, h2v{(_Float16)u, (_Float16)v});
     asm("" : "+v"(h));
     hi = as_h2(h);
-    lo = h2v{(_Float16)fmaf(x, f, -(float)hi.x), (_Float16)fmaf(y, g, -(float)hi.y)};
+    u = fmaf(x, f, -(float)hi.x), v = fmaf(y, g, -(float)hi.y);
+    asm("" : "+v"(u), "+v"(v));
+    lo = h2v{(_Float16)u, (_Float16)v};
 }
 
 // The same of single values.
@@ -321,51 +325,62 @@ struct Kv4Rows {
     f4v o[NG][2 * NB];
 };
 
-template <int NB, int NG>
-__device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn& a, int g, int row0, int R, int c, int L) {
+// A lane's elements of a row of q (of each block those of its group) and of the tables.
+template <int NB>
+struct Kv4Query {
+    float y[NB][8], cr[NB / 2][8], sr[NB / 2][8];
+    int at;   // the row's position
+};
+
+template <int NB>
+__device__ __forceinline__ void kv4_query(Kv4Query<NB>& x, const Kv4Attn& a, int g, int row, int L) {
+    const int t = kv4_token(a, row);
+    x.at = a.ctx - a.T + t;
+    const float* qp = a.q + (size_t)t * a.ldq + (g * a.rep + (row - t * a.rep)) * (32 * NB) + 8 * L;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-        const int row = min(row0 + 16 * n + c, R - 1);   // rows past the last one repeat it and are not stored
-        const int t = kv4_token(a, row), at = a.ctx - a.T + t;
-        const float* qp = a.q + (size_t)t * a.ldq + (g * a.rep + (row - t * a.rep)) * (32 * NB) + 8 * L;
-        float y[NB][8], x[NB][8], amax = 0.f;
+    for (int b = 0; b < NB; ++b) __builtin_memcpy(x.y[b], qp + 32 * b, 32);
+    if (!a.cos_t) return;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) __builtin_memcpy(y[b], qp + 32 * b, 32);
-        if (a.cos_t) {   // a pair's elements are half a head apart: both are the lane's
-#pragma unroll
-            for (int b = 0; b < NB / 2; ++b) {
-                float cr[8], sr[8];
-                __builtin_memcpy(cr, a.cos_t + (size_t)at * (16 * NB) + 32 * b + 8 * L, 32);
-                __builtin_memcpy(sr, a.sin_t + (size_t)at * (16 * NB) + 32 * b + 8 * L, 32);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) attn::rope2(y[b][e], y[b + NB / 2][e], cr[e], sr[e], &y[b][e], &y[b + NB / 2][e]);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = a.qsign * y[b][e];   // in the order of codes8
-#pragma unroll
-            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[b][e]));
-        }
-        amax = over_groups_max(amax);
-        const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 60);
-        const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-        r.factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            h2v hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(x[b][2 * e], up, x[b][2 * e + 1], up, hi[e], lo[e]);
-            r.qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
-            r.ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
-        }
-        r.seen[n] = at + 1;
-        r.m2[n] = kNegInf;
-        r.l[n] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) r.o[n][i] = f4v{};
+    for (int b = 0; b < NB / 2; ++b) {
+        __builtin_memcpy(x.cr[b], a.cos_t + (size_t)x.at * (16 * NB) + 32 * b + 8 * L, 32);
+        __builtin_memcpy(x.sr[b], a.sin_t + (size_t)x.at * (16 * NB) + 32 * b + 8 * L, 32);
     }
+}
+
+template <int NB, int NG>
+__device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn& a, Kv4Query<NB>& q, int n) {
+    float x[NB][8], amax = 0.f;
+    if (a.cos_t) {   // a pair's elements are half a head apart: both are the lane's
+#pragma unroll
+        for (int b = 0; b < NB / 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                attn::rope2(q.y[b][e], q.y[b + NB / 2][e], q.cr[b][e], q.sr[b][e], &q.y[b][e], &q.y[b + NB / 2][e]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[b][2 * (e & 3) + (e >> 2)] = q.y[b][e];   // in the order of codes8
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(q.y[b][e]));
+    }
+    amax = over_groups_max(amax);
+    const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 60);
+    const float up = a.qsign * __uint_as_float((uint32_t)(k + 127) << 23);
+    r.factor[n] = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        h2v hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split2(x[b][2 * e], up, x[b][2 * e + 1], up, hi[e], lo[e]);
+        r.qh[n][b] = h8_of(hi[0], hi[1], hi[2], hi[3]);
+        r.ql[n][b] = h8_of(lo[0], lo[1], lo[2], lo[3]);
+    }
+    r.seen[n] = q.at + 1;
+    r.m2[n] = kNegInf;
+    r.l[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) r.o[n][i] = f4v{};
 }
 
 // KG groups of 32 keys from key0 on; src: their operands (k, v) and scales (ks, vs) by
@@ -616,97 +631,31 @@ constexpr int kv4_part(int d) { return d + 4; }
 typedef unsigned int u4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u2v __attribute__((ext_vector_type(2)));
 
+// An offset that is past part_buffer's range for every size of a load: it answers 0.
+constexpr int kOutside = (int)0x80000000u;
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(const float* part) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, 0x7fffffff, 0x00020000);
 }
 
-// out[row] = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the nch chunks of `rows`
-// rows, by a workgroup of 512.  A thread takes four elements of a row, and where rows
-// are few several threads share the chunks: c, c + P, ..., eight at a time whose loads
-// are all issued before any is used; they merge through LDS.  row_at: the row's place.
-// COHERENT: the partials were written by other workgroups of the launch.
-template <int D>
-struct Kv4MergeLds {
-    float4 o[512];
-    float m[512], l[512];
-};
-
-template <int D, bool COHERENT, class At>
-__device__ __forceinline__ void kv4_merge(Kv4MergeLds<D>& sm, const float* part, int nch, int rows, float* out,
-                                          uint16_t* out16, At row_at) {
-    constexpr int B = 8, Q = D / 4, PS = kv4_part(D), AUX = COHERENT ? 16 : 0;   // 16: sc1, past this die's L2
-    const int n = rows * Q, P = 512 / n, tid = threadIdx.x, share = tid / n, i = tid - share * n;
-    const bool on = share < P;
-    const size_t at = row_at(on ? i / Q : 0);
-    const auto pr = part_buffer(part);
-    const int first = (int)(4 * at * nch * PS);
-    float M = kNegInf, sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (on) {
-        for (int c0 = share; c0 < nch; c0 += B * P) {
-            float pm[B], pl[B], mb = M;
-            float4 po[B];
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const int x = first + 4 * min(c0 + b * P, nch - 1) * PS;
-                const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, x + 4 * D, 0, AUX));
-                pm[b] = ml.x;
-                pl[b] = ml.y;
-                po[b] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(pr, x + 16 * (i % Q), 0, AUX));
-            }
-#pragma unroll
-            for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
-            const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
-            sum *= f;
-            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const float e = c0 + b * P < nch && pm[b] != kNegInf ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
-                sum = fmaf(e, pl[b], sum);
-                o.x = fmaf(e, po[b].x, o.x); o.y = fmaf(e, po[b].y, o.y); o.z = fmaf(e, po[b].z, o.z); o.w = fmaf(e, po[b].w, o.w);
-            }
-            M = mb;
-        }
-    }
-    if (P > 1) {
-        sm.m[tid] = M;
-        sm.l[tid] = sum;
-        sm.o[tid] = o;
-        __syncthreads();
-        if (share) return;
-        const float m0 = M;
-        for (int k = 1; k < P; ++k) M = fmaxf(M, sm.m[i + k * n]);
-        const float f0 = m0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
-        sum *= f0;
-        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-        for (int k = 1; k < P; ++k) {
-            const float mk = sm.m[i + k * n], f = mk == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mk - M);
-            const float4 x = sm.o[i + k * n];
-            sum = fmaf(f, sm.l[i + k * n], sum);
-            o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
-        }
-    }
-    if (!on || share) return;
-    const float by = sum == 0.f ? 0.f : 1.f / sum;
-    const float x[4] = {o.x * by, o.y * by, o.z * by, o.w * by};
-    kv4_store(out, out16, at * D + 4 * (i % Q), x);
-}
+// The last workgroup of a block merges its chunks, up to 32 of them; more are merged by a launch
+// of their own, a workgroup a row.  In the launch / in one of its own, us: 16 chunks (32/4 heads of 64, 4096
+// keys) 8.1 / 9.4, 32 (32/8 of 128, 15001) 12.5 / 13.3, 59 (8/1 of 128, 15001) 12.9 / 10.3, 235 (60001)
+// 26.5 / 11.9.
+constexpr int kMergedChunks = 32;
 
 constexpr int kWaves = 8;   // of a workgroup of 16 rows
 
 template <int D>
 struct Kv4WavesLds {
-    float o[kWaves][16 * (D + 4)], m[kWaves][16], l[kWaves][16], f[kWaves][16];
+    float o[kWaves][16 * (D + 4)], m[16][kWaves], l[16][kWaves];
 };
 
 template <int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
     constexpr int NB = D / 32, NG = 1, ROWS = 16 * NG, OS = D + 4;
     __shared__ int last;
-    __shared__ __align__(16) union Lds {   // the chunks are merged after the waves
-        Kv4WavesLds<D> waves;
-        Kv4MergeLds<D> merge;
-    } lds;
+    __shared__ __align__(16) Kv4WavesLds<D> x;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
     if (a.pos_dev) a.ctx = min(*a.pos_dev + 1, a.ctx);
     const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, row0 = blockIdx.z * ROWS, R = a.T * a.rep;
@@ -722,8 +671,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     Kv4Raw<NB> raw;
     raw.magic = magic1024();
     if (mine > 0) kv4_load<NB>(raw, kc, vc, ks, vs, kb0, c, L);
+    Kv4Query<NB> q;
+    kv4_query<NB>(q, a, g, min(row0 + c, R - 1), L);   // rows past the last one repeat it and are not stored
     Kv4Rows<NB, NG> r;
-    kv4_rows_init<NB, NG>(r, a, g, row0, R, c, L);
+    kv4_rows_init<NB, NG>(r, a, q, 0);
     // Three loops of one body each (two in one would cost each other registers): the groups
     // that every row sees whole, those at some row's edge, and those of both that the first
     // two left because of a large scale.
@@ -755,11 +706,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
         }
 
     // ---- the waves' results, then the chunk's ----
-    Kv4WavesLds<D>& x = lds.waves;
     const float sum = over_groups_sum(r.l[0]);
     if (L == 0) {
-        x.m[w][c] = sum != sum ? INFINITY : r.m2[0];   // a NaN has to win where the others' weights would drop it
-        x.l[w][c] = sum;
+        x.m[c][w] = sum != sum ? INFINITY : r.m2[0];   // a NaN has to win where the others' weights would drop it
+        x.l[c][w] = sum;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)   // rows 4L + j of the two tiles: elements 8L + 2j and 8L + 2j + 1 of the block
@@ -769,23 +719,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
                 make_float4(r.o[0][2 * b][2 * h], r.o[0][2 * b + 1][2 * h], r.o[0][2 * b][2 * h + 1], r.o[0][2 * b + 1][2 * h + 1]);
     __syncthreads();
     const int rows = min(ROWS, R - row0), tid = threadIdx.x;
-    if (tid < 16 * kWaves) {
-        const int k = tid >> 4, j = tid & 15;
-        float M = x.m[0][j];
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) M = fmaxf(M, x.m[i][j]);
-        x.f[k][j] = x.m[k][j] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.m[k][j] - M);
-    }
-    __syncthreads();
     for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
         const int j = i / (D / 4), e = 4 * (i % (D / 4));
-        float M = x.m[0][j], l = 0.f, v[4] = {};
+        float m[kWaves], M = kNegInf, l = 0.f, v[4] = {};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) M = fmaxf(M, m[k] = x.m[j][k]);
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            const float f = x.f[k][j];
+            const float f = m[k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[k] - M);
             const float4 y = *reinterpret_cast<const float4*>(&x.o[k][j * OS + e]);
-            M = fmaxf(M, x.m[k][j]);
-            l = fmaf(f, x.l[k][j], l);
+            l = fmaf(f, x.l[j][k], l);
             v[0] = fmaf(f, y.x, v[0]); v[1] = fmaf(f, y.y, v[1]); v[2] = fmaf(f, y.z, v[2]); v[3] = fmaf(f, y.w, v[3]);
         }
         const size_t at = kv4_row(a, g, row0 + j);
@@ -814,7 +757,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     }
     __syncthreads();
     if (!last) return;
-    kv4_merge<D, true>(lds.merge, a.part, nch, rows, a.out, a.out16, [&](int j) { return kv4_row(a, g, row0 + j); });
+    // A wave a row, in few instructions: they run once, from a cold cache.  Lane i weighs chunk
+    // i; the wave's halves (quarters where D is 64) take every second (fourth) chunk's O,
+    // all loads at once.  What lies past the last chunk reads as 0, out of the buffer's range.
+    constexpr int Q = D / 4, SHARES = 64 / Q, EACH = kMergedChunks / SHARES, PS = kv4_part(D);
+    const auto pr = part_buffer(a.part);
+    const int e = 4 * (lane % Q), share = lane / Q;
+    for (int j = w; j < rows; j += kWaves) {
+        const size_t at = kv4_row(a, g, row0 + j);
+        const int first = (int)(4 * at * nch * PS);
+        const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, lane < nch ? first + 4 * (lane * PS + D) : kOutside, 0, 16));
+        f4v y[EACH], o = {};
+        auto ask = [&](int from) {
+#pragma unroll
+            for (int i = from; i < from + EACH / 2; ++i) {
+                const int k = share + i * SHARES;
+                y[i] = __builtin_bit_cast(f4v, __builtin_amdgcn_raw_buffer_load_b128(pr, k < nch ? first + 4 * (k * PS + e) : kOutside, 0, 16));
+            }
+        };
+        ask(0);
+        const bool more = nch > EACH / 2 * SHARES;
+        if (more) ask(EACH / 2);
+        const float m = lane < nch ? ml.x : kNegInf, M = wave_max(m);
+        const float f = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - M), l = wave_sum(f * ml.y);
+        auto add = [&](int from) {
+#pragma unroll
+            for (int i = from; i < from + EACH / 2; ++i) o += __shfl(f, share + i * SHARES) * y[i];
+        };
+        add(0);
+        if (more) add(EACH / 2);
+        const float by = l == 0.f ? 0.f : 1.f / l;
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float2 t = swap_halves32(o[i], o[i]);
+            v[i] = t.x + t.y;
+            if (SHARES == 4) {
+                t = swap_rows16(v[i], v[i]);
+                v[i] = t.x + t.y;
+            }
+            v[i] *= by;
+        }
+        if (share == 0) kv4_store(a.out, a.out16, at * D + e, v);
+    }
 }
 
 // ---- many rows --------------------------------------------------------------------
@@ -960,7 +945,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     auto is_large = [&]() { return __builtin_amdgcn_readfirstlane(st.large[0] | st.large[1] | st.large[2] | st.large[3]) != 0; };
 
     Kv4Rows<NB, NG> r;
-    kv4_rows_init<NB, NG>(r, a, g, min(row0, R - 1), R, c, L);
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        Kv4Query<NB> q;
+        kv4_query<NB>(q, a, g, min(row0 + 16 * n + c, R - 1), L);   // rows past the last one repeat it and are not stored
+        kv4_rows_init<NB, NG>(r, a, q, n);
+    }
     bool left = false;
     stages(std::false_type(), 0, inside, [&](int s) {
         if (is_large()) {
@@ -1010,11 +1000,61 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
 }
 
 // The merge as a launch of its own: a row a workgroup.
+// out[row] = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M) l_c over the nch chunks of a row.  A
+// thread takes four elements of every P-th chunk, eight at a time whose loads are all issued
+// before any is used; they merge through LDS.
 template <int D>
 __global__ __launch_bounds__(512) void kv4_merge_kernel(const float* __restrict__ part, int nch, float* __restrict__ out,
                                                         uint16_t* __restrict__ out16) {
-    __shared__ Kv4MergeLds<D> sm;
-    kv4_merge<D, false>(sm, part, nch, 1, out, out16, [](int) { return (size_t)blockIdx.x; });
+    constexpr int B = 8, Q = D / 4, P = 512 / Q, PS = kv4_part(D);
+    __shared__ float4 so[512];
+    __shared__ float sm[P], sl[P];
+    const int tid = threadIdx.x, share = tid / Q, i = tid % Q;
+    const float* row = part + (size_t)blockIdx.x * nch * PS;
+    float M = kNegInf, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = share; c0 < nch; c0 += B * P) {
+        float pm[B], pl[B], mb = M;
+        float4 po[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const float* x = row + min(c0 + b * P, nch - 1) * PS;
+            pm[b] = x[D];
+            pl[b] = x[D + 1];
+            po[b] = *reinterpret_cast<const float4*>(x + 4 * i);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) mb = fmaxf(mb, pm[b]);   // a repeated last chunk does no harm
+        const float f = M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+        sum *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const float e = c0 + b * P < nch && pm[b] != kNegInf ? __builtin_amdgcn_exp2f(pm[b] - mb) : 0.f;
+            sum = fmaf(e, pl[b], sum);
+            o.x = fmaf(e, po[b].x, o.x); o.y = fmaf(e, po[b].y, o.y); o.z = fmaf(e, po[b].z, o.z); o.w = fmaf(e, po[b].w, o.w);
+        }
+        M = mb;
+    }
+    so[tid] = o;
+    if (i == 0) {
+        sm[share] = M;
+        sl[share] = sum;
+    }
+    __syncthreads();
+    if (share) return;
+    for (int k = 0; k < P; ++k) M = fmaxf(M, sm[k]);
+    float l = 0.f, v[4] = {};
+    for (int k = 0; k < P; ++k) {
+        const float f = sm[k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(sm[k] - M);
+        const float4 x = so[k * Q + i];
+        l = fmaf(f, sl[k], l);
+        v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
+    }
+    const float by = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= by;
+    kv4_store(out, out16, (size_t)blockIdx.x * D + 4 * i, v);
 }
 
 }  // namespace
@@ -1107,11 +1147,6 @@ Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
     return p;
 }
 
-// The last workgroup of a block merges its chunks, up to 32 of them; more are merged by a launch
-// of their own, a workgroup a row.  In the launch / in one of its own, us: 16 chunks (32/4 heads of 64, 4096
-// keys) 8.1 / 9.4, 32 (32/8 of 128, 15001) 12.5 / 13.3, 59 (8/1 of 128, 15001) 12.9 / 10.3, 235 (60001)
-// 26.5 / 11.9.
-constexpr int kMergedChunks = 32;
 static_assert(kSharers <= kSmallMaxTiles, "a counter for each block whose keys are shared");
 }  // namespace
 
