@@ -197,10 +197,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // share a block's keys: the eight waves of each take groups of 32 keys in turn, each
 // with its own running maximum and sum, and merge through LDS, and the workgroup that
 // comes last merges all of a block's.
-// One decode row at 32/8 heads of 128: 120001 keys 42 us (138 MB, 3.3 TB/s with the
-// launch, its first loads and the merge: 4.0 TB/s without, what a large read reaches),
-// 15001 keys 12 (17 MB: 1.4 TB/s; bound by that chain of waits, two groups a wave); 4096
-// keys at 32/4 heads of 64 8 us.
+// One decode row at 32/8 heads of 128: 120001 keys 34.5 us (138 MB, 4.0 TB/s, what a large
+// read reaches); 15001 keys 10.0 (17 MB, 1.7 TB/s) and 1500 keys 6.8, bound by the chain of
+// waits: the launch, the arguments, q and the keys, the group's products and weights, the waves'
+// merge, the counter, the chunks' merge, 0.3 to 0.9 us each.
 //   scores   S^T = K Q^T, 16 keys by 16 rows and a block of 32 elements an
 //            instruction.  A code minus 8 is exact in f16; q, scaled by a power of
 //            two for the row's largest element to lie in [2^13, 2^14), enters as two
@@ -383,17 +383,61 @@ __device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn&
     for (int i = 0; i < 2 * NB; ++i) r.o[n][i] = f4v{};
 }
 
+// How far a block's products are formed below: the exponent, over 2^0, of the largest finite
+// scale of V among the 32 keys.
+__device__ __forceinline__ int kv4_down(const uint4& vs) {
+    uint32_t top = 15;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t x = (word_of(vs, j >> 1) >> (16 * (j & 1) + 10)) & 31u;
+        top = x < 31u ? max(top, x) : top;
+    }
+    return (int)over_groups_max((float)top) - 15;
+}
+
 // KG groups of 32 keys from key0 on; src: their operands (k, v) and scales (ks, vs) by
 // group and block.  kEdge: some row does not see all of them; kApart: as well, a value
 // block's scale is 2 or more (or no number).
 enum { kInside, kEdge, kApart };
+
+// A row's scores of KG groups of 32 keys, the lane's, become weights; m2 and l move on, and the
+// factor that O so far takes is returned.  end: the first key, from the lane's first one
+// on, that the row does not see.
+template <int MODE, int KG>
+__device__ __forceinline__ float kv4_weights(float (&s)[KG][8], float factor, int end, float& m2, float& l) {
+    float mx = kNegInf;
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (MODE != kInside) s[kg][e] = 32 * kg + kv4::key_of(0, e) >= end ? kNegInf : s[kg][e];
+            mx = fmaxf(mx, s[kg][e]);
+        }
+    mx = over_groups_max(mx);
+    mx = mx == kNegInf ? kNegInf : mx * factor;
+    const bool grow = mx > m2 + kHeadroom;
+    const float mn = grow ? mx : m2;
+    const float corr = grow ? __builtin_amdgcn_exp2f(m2 - mn) : 1.f;
+    m2 = mn;
+    const float at = mn == kNegInf ? 0.f : kWeightBits - mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            s[kg][e] = __builtin_amdgcn_exp2f(fmaf(s[kg][e], factor, at));   // 0 of -inf: the factor is positive
+            sum += s[kg][e];
+        }
+    l = fmaf(l, corr, sum);
+    return corr;
+}
 
 template <int MODE, int KG, int NB, int NG, class Src>
 __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int key0, int L) {
     // ---- scores: slots 4u + j of the lane's keys ----
     // The next half group's operands are read before this one's products (LDS takes longer
     // than a few of those); the barriers hold the order.
-    float s[KG][NG][8];
+    float s[NG][KG][8];
     h8v ka[2][NB];
     h2v dk[2][NB][2];
     auto read = [&](int i) {   // half group i
@@ -422,7 +466,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float& x = s[i >> 1][n][4 * (i & 1) + j];
+                    float& x = s[n][i >> 1][4 * (i & 1) + j];
                     const h2v d = dk[i & 1][b][j >> 1];
                     x = fmaf(t[b][j], (float)((j & 1) ? d.y : d.x), b == 0 ? 0.f : x);
                 }
@@ -432,33 +476,9 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
     if (Src::kValues) __builtin_amdgcn_s_setprio(1);   // the other wave's products run under this one's softmax
     __builtin_amdgcn_sched_barrier(0);   // no loads of the next part early: they would cost registers
     // ---- softmax ----
-    auto hidden = [&](int kg, int n, int e) { return 32 * kg + kv4::key_of(0, e) >= r.seen[n] - key0 - 4 * L; };
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-        float mx = kNegInf;
-#pragma unroll
-        for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (MODE != kInside) s[kg][n][e] = hidden(kg, n, e) ? kNegInf : s[kg][n][e];
-                mx = fmaxf(mx, s[kg][n][e]);
-            }
-        mx = over_groups_max(mx);
-        mx = mx == kNegInf ? kNegInf : mx * r.factor[n];
-        const bool grow = mx > r.m2[n] + kHeadroom;
-        const float mn = grow ? mx : r.m2[n];
-        const float corr = grow ? __builtin_amdgcn_exp2f(r.m2[n] - mn) : 1.f;
-        r.m2[n] = mn;
-        const float at = mn == kNegInf ? 0.f : kWeightBits - mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int kg = 0; kg < KG; ++kg)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                s[kg][n][e] = __builtin_amdgcn_exp2f(fmaf(s[kg][n][e], r.factor[n], at));   // 0 of -inf: the factor is positive
-                sum += s[kg][n][e];
-            }
-        r.l[n] = fmaf(r.l[n], corr, sum);
+        const float corr = kv4_weights<MODE, KG>(s[n], r.factor[n], r.seen[n] - key0 - 4 * L, r.m2[n], r.l[n]);
         // Without a branch around it, although corr is 1 most of the time: the branch keeps
         // O in registers twice.
 #pragma unroll
@@ -477,7 +497,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int e = 4 * (i >> 1) + (i & 1);
-                split2(s[kg][n][e], s[kg][n][e + 2], hi[i], lo[i]);
+                split2(s[n][kg][e], s[n][kg][e + 2], hi[i], lo[i]);
             }
             ph[kg][n] = h8_of(hi[0], hi[1], hi[2], hi[3]);
             pl[kg][n] = h8_of(lo[0], lo[1], lo[2], lo[3]);
@@ -509,15 +529,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
             src.v(kg, b, va, wa);
             const uint4 vs = src.vs(kg, b);
             int down = 0;                                // powers of two that the block's products are formed below
-            if constexpr (MODE == kApart) {
-                uint32_t top = 15;                       // the largest exponent of the finite scales
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t x = (word_of(vs, j >> 1) >> (16 * (j & 1) + 10)) & 31u;
-                    top = x < 31u ? max(top, x) : top;
-                }
-                down = (int)over_groups_max((float)top) - 15;
-            }
+            if constexpr (MODE == kApart) down = kv4_down(vs);
             const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -528,10 +540,10 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
                 for (int i = 0; i < 4; ++i) {
                     const int e = 4 * (i >> 1) + (i & 1);
                     const h2v d0 = as_h2(word_of(vs, e >> 1)), d1 = as_h2(word_of(vs, (e >> 1) + 1));
-                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[kg][n][e], p1 = s[kg][n][e + 2];
+                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[n][kg][e], p1 = s[n][kg][e + 2];
                     if constexpr (MODE == kApart) {
-                        f = hidden(kg, n, e) ? 0.f : f;
-                        g = hidden(kg, n, e + 2) ? 0.f : g;
+                        f = 32 * kg + kv4::key_of(0, e) >= r.seen[n] - key0 - 4 * L ? 0.f : f;
+                        g = 32 * kg + kv4::key_of(0, e + 2) >= r.seen[n] - key0 - 4 * L ? 0.f : g;
                         p0 *= scale_down;
                         p1 *= scale_down;
                     }
@@ -558,11 +570,11 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
 
 // A wave's share of 32 keys as it is loaded: lane (c, L) holds K words of keys c and
 // 16 + c, V bytes of elements 2c, 2c + 1 of each block for the keys of group L, and
-// those keys' scales.
-template <int NB>
+// those keys' scales, of NS blocks: all, or the one that the lane's column stands for.
+template <int NB, int NS = NB>
 struct Kv4Raw {
     uint32_t kw[2][NB], vw[2 * NB];
-    uint4 kd[NB], vd[NB];
+    uint4 kd[NS], vd[NS];
     uint32_t magic;
     static constexpr bool kValues = false;
 
@@ -608,21 +620,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t group_buffer(const T* p, int b
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, bytes, 0x00020000);
 }
 
-template <int NB>
-__device__ __forceinline__ void kv4_load(Kv4Raw<NB>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks,
-                                         const uint16_t* vs, int kb, int c, int L) {
+template <int NB, int NS>
+__device__ __forceinline__ void kv4_load(Kv4Raw<NB, NS>& r, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks,
+                                         const uint16_t* vs, int kb, int c, int L, int own) {
     constexpr int D = 32 * NB, CODES = kv4::kKeys * D / 2;
     const auto kr = group_buffer(kc + (size_t)kb * CODES, CODES), vr = group_buffer(vc + (size_t)kb * CODES, CODES);
     const auto sr = group_buffer(ks + (size_t)kb * D, 2 * D), tr = group_buffer(vs + (size_t)kb * D, 2 * D);
 #pragma unroll
     for (int u = 0; u < 2; ++u) buffer_words<NB>(r.kw[u], kr, (c + 16 * u) * (D / 2) + 4 * L * NB);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-        r.kd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (L * NB + b), 0, 0));
+    for (int b = 0; b < NS; ++b)
+        r.kd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sr, 16 * (L * NB + own + b), 0, 0));
     buffer_words<2 * NB>(r.vw, vr, (L * 16 + c) * 8 * NB);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-        r.vd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + b), 0, 0));
+    for (int b = 0; b < NS; ++b)
+        r.vd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + own + b), 0, 0));
 }
 
 // A chunk's partial of a row: acc[D], m, l and two floats that align the next.  The host
@@ -638,25 +650,156 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(const float* part)
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, 0x7fffffff, 0x00020000);
 }
 
-// The last workgroup of a block merges its chunks, up to 32 of them; more are merged by a launch
-// of their own, a workgroup a row.  In the launch / in one of its own, us: 16 chunks (32/4 heads of 64, 4096
-// keys) 8.1 / 9.4, 32 (32/8 of 128, 15001) 12.5 / 13.3, 59 (8/1 of 128, 15001) 12.9 / 10.3, 235 (60001)
-// 26.5 / 11.9.
+// The last workgroup of a block merges its chunks, up to 32 of them (all that its lanes ask
+// for at once); more are merged by a launch of their own, a workgroup a row.  In the launch
+// / in one of its own, us: 16 chunks (32/4 heads of 64, 4096 keys) 6.3 / 8.0, 6 (32/8 of 128, 1500) 6.8
+// / 8.1, 32 (15001) 10.0 / 11.3, 32 (120001) 34.2 / 36.3, 3 (40 rows of 3001) 16.4 / 18.0; a merge in
+// the launch of any number took, 59 chunks (8/1 of 128, 15001), 12.9 / 10.3, 235 (60001) 26.5 / 11.9.
 constexpr int kMergedChunks = 32;
+
+// ---- few rows ---------------------------------------------------------------------
+// Where a KV head's rows are 16 / NB or fewer (a decode step of a usual group) the 16
+// columns stand for its rows and blocks: column NB row + b has the row's q where its block
+// is b, zeros elsewhere, and the weights times b's scales of V.  So a lane loads, splits and
+// scales one block of q and of the scales instead of all, which is most of the work of a
+// group of keys; the columns' scores of a row are summed by exchanges within four lanes,
+// and of each block's product O the column with the block's own scales is kept.  One
+// row of 1500, 15001 and 120001 keys at 32/8 heads of 128: 7.9, 11.4 and 40 us with a column
+// a row, 6.8, 10.0 and 34.5 so; 4096 keys at 32/4 of 64 6.6 and 6.3.
+template <int NB>
+struct Kv4Few {
+    h8v qh[NB], ql[NB];
+    float factor, m2, l;
+    int seen;
+    f4v o[2 * NB];
+};
+
+template <int NB>
+__device__ __forceinline__ float over_blocks_max(float v) {
+    v = fmaxf(v, quad_f(v, 1));
+    return NB == 4 ? fmaxf(v, quad_f(v, 2)) : v;
+}
+
+template <int NB>
+__device__ __forceinline__ float over_blocks_sum(float v) {
+    v += quad_f(v, 1);
+    return NB == 4 ? v + quad_f(v, 2) : v;
+}
+
+// b: the lane's block.
+template <int NB>
+__device__ __forceinline__ void kv4_few_init(Kv4Few<NB>& r, const Kv4Attn& a, int g, int row, int b, int L) {
+    const int t = kv4_token(a, row), at = a.ctx - a.T + t;
+    const float* qp = a.q + (size_t)t * a.ldq + (g * a.rep + (row - t * a.rep)) * (32 * NB) + 8 * L;
+    float y[8], amax = 0.f;
+    __builtin_memcpy(y, qp + 32 * b, 32);
+    if (a.cos_t) {
+        const bool first = b < NB / 2;   // of a pair, whose elements are half a head apart
+        const int i = first ? b : b - NB / 2;
+        float x[8], cr[8], sr[8];
+        __builtin_memcpy(x, qp + 32 * (first ? b + NB / 2 : i), 32);
+        __builtin_memcpy(cr, a.cos_t + (size_t)at * (16 * NB) + 32 * i + 8 * L, 32);
+        __builtin_memcpy(sr, a.sin_t + (size_t)at * (16 * NB) + 32 * i + 8 * L, 32);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u, v;
+            attn::rope2(first ? y[e] : x[e], first ? x[e] : y[e], cr[e], sr[e], &u, &v);
+            y[e] = first ? u : v;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
+    amax = over_blocks_max<NB>(over_groups_max(amax));
+    const int k = min(140 - (int)(__float_as_uint(amax) >> 23), 60);
+    const float up = a.qsign * __uint_as_float((uint32_t)(k + 127) << 23);
+    r.factor = a.sl2 * __uint_as_float((uint32_t)(127 - k) << 23);
+    h2v hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2(y[e], up, y[e + 4], up, hi[e], lo[e]);   // in the order of codes8
+    const h8v qh = h8_of(hi[0], hi[1], hi[2], hi[3]), ql = h8_of(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        r.qh[i] = i == b ? qh : h8v{};
+        r.ql[i] = i == b ? ql : h8v{};
+    }
+    r.seen = at + 1;
+    r.m2 = kNegInf;
+    r.l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) r.o[i] = f4v{};
+}
+
+template <int MODE, int NB>
+__device__ __forceinline__ void kv4_few_keys(Kv4Few<NB>& r, const Kv4Raw<NB, 1>& x, int key0, int L) {
+    f4v t[2] = {};
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const h8v k = x.k(0, u, b);
+            t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, r.ql[b], t[u], 0, 0, 0);
+            t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, r.qh[b], t[u], 0, 0, 0);
+        }
+    float s[1][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const h2v d = as_h2(word_of(x.kd[0], e >> 1));
+        s[0][e] = over_blocks_sum<NB>(t[e >> 2][e & 3] * (float)((e & 1) ? d.y : d.x));
+    }
+    const float corr = kv4_weights<MODE, 1>(s, r.factor, r.seen - key0 - 4 * L, r.m2, r.l);
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) r.o[i] *= corr;
+    int down = 0;   // powers of two that the column's products are formed below
+    if constexpr (MODE == kApart) down = kv4_down(x.vd[0]);
+    const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23), back = __uint_as_float((uint32_t)(127 + down) << 23);
+    h2v hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand
+        const int e = 4 * (i >> 1) + (i & 1);
+        const h2v d0 = as_h2(word_of(x.vd[0], e >> 1)), d1 = as_h2(word_of(x.vd[0], (e >> 1) + 1));
+        float f = (i & 1) ? d0.y : d0.x, h = (i & 1) ? d1.y : d1.x, p0 = s[0][e], p1 = s[0][e + 2];
+        if constexpr (MODE == kApart) {   // a key that the row does not see weighs 0 whatever its scale is
+            f = kv4::key_of(0, e) >= r.seen - key0 - 4 * L ? 0.f : f;
+            h = kv4::key_of(0, e + 2) >= r.seen - key0 - 4 * L ? 0.f : h;
+            p0 *= scale_down;
+            p1 *= scale_down;
+        }
+        split2(p0, f, p1, h, hi[i], lo[i]);
+    }
+    const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        h8v v[2];   // even elements, odd elements
+        x.v(0, b, v[0], v[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f4v& o = r.o[2 * b + h];
+            if constexpr (MODE == kApart) {
+                f4v y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], pl, f4v{}, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], ph, y, 0, 0, 0);
+                o += y * back;
+            } else {
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], pl, o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[h], ph, o, 0, 0, 0);
+            }
+        }
+    }
+}
 
 constexpr int kWaves = 8;   // of a workgroup of 16 rows
 
-template <int D>
+template <int D, int ROWS>
 struct Kv4WavesLds {
-    float o[kWaves][16 * (D + 4)], m[16][kWaves], l[16][kWaves];
+    float o[kWaves][ROWS * (D + 4)], m[ROWS][kWaves], l[ROWS][kWaves];
 };
 
-template <int D>
+template <int D, bool FEW>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
-    constexpr int NB = D / 32, NG = 1, ROWS = 16 * NG, OS = D + 4;
+    constexpr int NB = D / 32, ROWS = FEW ? 16 / NB : 16, OS = D + 4;
     __shared__ int last;
-    __shared__ __align__(16) Kv4WavesLds<D> x;
+    __shared__ __align__(16) Kv4WavesLds<D, ROWS> x;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
+    const int lane_row = FEW ? c / NB : c, own = FEW ? c % NB : 0;   // the lane's row, its block
     if (a.pos_dev) a.ctx = min(*a.pos_dev + 1, a.ctx);
     const int nch = a.nch, chunk = blockIdx.x, g = blockIdx.y, row0 = blockIdx.z * ROWS, R = a.T * a.rep;
     const uint8_t *kc = a.kc + g * a.codes, *vc = a.vc + g * a.codes;
@@ -668,55 +811,86 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     auto mine_of = [&](int groups) { return groups > kb0 ? (groups - kb0 + stride - 1) / stride : 0; };
     const int mine = mine_of((most + kv4::kKeys - 1) / kv4::kKeys), inside = min(mine, mine_of(fewest / kv4::kKeys));
 
-    Kv4Raw<NB> raw;
+    using Raw = Kv4Raw<NB, FEW ? 1 : NB>;
+    Raw raw;
     raw.magic = magic1024();
-    if (mine > 0) kv4_load<NB>(raw, kc, vc, ks, vs, kb0, c, L);
-    Kv4Query<NB> q;
-    kv4_query<NB>(q, a, g, min(row0 + c, R - 1), L);   // rows past the last one repeat it and are not stored
-    Kv4Rows<NB, NG> r;
-    kv4_rows_init<NB, NG>(r, a, q, 0);
+    if (mine > 0) kv4_load(raw, kc, vc, ks, vs, kb0, c, L, own);
+    __builtin_amdgcn_sched_barrier(0);
+    std::conditional_t<FEW, Kv4Few<NB>, Kv4Rows<NB, 1>> r;
+    const int row = min(row0 + lane_row, R - 1);   // rows past the last one repeat it and are not stored
+    if constexpr (FEW) {
+        kv4_few_init(r, a, g, row, own, L);
+    } else {
+        Kv4Query<NB> q;
+        kv4_query(q, a, g, row, L);
+        kv4_rows_init(r, a, q, 0);
+    }
+    auto keys = [&](auto mode, const Raw& x, int i) {
+        const int key0 = (kb0 + i * stride) * kv4::kKeys;
+        if constexpr (FEW) kv4_few_keys<mode.value>(r, x, key0, L);
+        else kv4_keys<mode.value, 1>(r, x, key0, L);
+    };
+    constexpr std::integral_constant<int, kInside> whole;
+    constexpr std::integral_constant<int, kEdge> edge;
+    constexpr std::integral_constant<int, kApart> apart;
     // Three loops of one body each (two in one would cost each other registers): the groups
     // that every row sees whole, those at some row's edge, and those of both that the first
     // two left because of a large scale.
     bool left = false;
-    auto large = [&](const Kv4Raw<NB>& x) {   // a scale of 2 or more, or no number
+    auto large = [&](const Raw& x) {   // a scale of 2 or more, or no number
         uint32_t any = 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) any |= x.vd[b].x | x.vd[b].y | x.vd[b].z | x.vd[b].w;
+        for (int b = 0; b < (FEW ? 1 : NB); ++b) any |= x.vd[b].x | x.vd[b].y | x.vd[b].z | x.vd[b].w;
         return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
     };
-    auto load = [&](int i) { kv4_load<NB>(raw, kc, vc, ks, vs, kb0 + i * stride, c, L); };   // i < mine
+    auto load = [&](int i) { kv4_load(raw, kc, vc, ks, vs, kb0 + i * stride, c, L, own); };   // i < mine
     int i = 0;
     for (; i < inside; ++i) {
-        const Kv4Raw<NB> cur = raw;
+        const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
         if (large(cur)) left = true;
-        else kv4_keys<kInside, 1>(r, cur, (kb0 + i * stride) * kv4::kKeys, L);
+        else keys(whole, cur, i);
     }
     for (; i < mine; ++i) {
-        const Kv4Raw<NB> cur = raw;
+        const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
         if (large(cur)) left = true;
-        else kv4_keys<kEdge, 1>(r, cur, (kb0 + i * stride) * kv4::kKeys, L);
+        else keys(edge, cur, i);
     }
     if (left)
         for (i = 0; i < mine; ++i) {
             load(i);
-            if (large(raw)) kv4_keys<kApart, 1>(r, raw, (kb0 + i * stride) * kv4::kKeys, L);
+            if (large(raw)) keys(apart, raw, i);
         }
 
     // ---- the waves' results, then the chunk's ----
-    const float sum = over_groups_sum(r.l[0]);
-    if (L == 0) {
-        x.m[c][w] = sum != sum ? INFINITY : r.m2[0];   // a NaN has to win where the others' weights would drop it
-        x.l[c][w] = sum;
+    float l, m;
+    if constexpr (FEW) l = r.l, m = r.m2;
+    else l = r.l[0], m = r.m2[0];
+    l = over_groups_sum(l);
+    if (L == 0 && own == 0) {
+        x.m[lane_row][w] = l != l ? INFINITY : m;   // a NaN has to win where the others' weights would drop it
+        x.l[lane_row][w] = l;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b)   // rows 4L + j of the two tiles: elements 8L + 2j and 8L + 2j + 1 of the block
+    // Rows 4L + j of a block's two tiles: its elements 8L + 2j and 8L + 2j + 1.
+    auto put = [&](int b, const f4v& even, const f4v& odd) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float4*>(&x.o[w][c * OS + 32 * b + 8 * L + 4 * h]) =
-                make_float4(r.o[0][2 * b][2 * h], r.o[0][2 * b + 1][2 * h], r.o[0][2 * b][2 * h + 1], r.o[0][2 * b + 1][2 * h + 1]);
+            *reinterpret_cast<float4*>(&x.o[w][lane_row * OS + 32 * b + 8 * L + 4 * h]) =
+                make_float4(even[2 * h], odd[2 * h], even[2 * h + 1], odd[2 * h + 1]);
+    };
+    if constexpr (FEW) {
+        f4v even = r.o[0], odd = r.o[1];
+#pragma unroll
+        for (int b = 1; b < NB; ++b) {
+            even = own == b ? r.o[2 * b] : even;
+            odd = own == b ? r.o[2 * b + 1] : odd;
+        }
+        put(own, even, odd);
+    } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) put(b, r.o[0][2 * b], r.o[0][2 * b + 1]);
+    }
     __syncthreads();
     const int rows = min(ROWS, R - row0), tid = threadIdx.x;
     for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
@@ -1121,6 +1295,7 @@ int launch_kv4_dequant(hipStream_t s, const KVLayer& L, int n_kv, int d_head, in
 namespace {
 struct Kv4Plan {
     bool tiles = false;                      // the kernel for many rows
+    bool few = false;                        // the kernel for a column a row and block
     int blocks = 1, nch = 1;                 // blocks of rows of a KV head, workgroups that share a block's keys
 };
 
@@ -1128,12 +1303,12 @@ struct Kv4Plan {
 // time): 1777 rows of 4001 keys at 32/8 heads of 128 (448 workgroups) 406 / 228 us, 1024 of 1024
 // (256) 76 / 60, 1024 of 2048 at 32/4 of 64 (256) 64 / 63; but 700 of 4000 (176) 197 / 206, 512 of
 // 1024 (128) 46 / 57.  Below, blocks of 16 rows, whose keys are shared out to as many
-// workgroups as there are CUs, one group of keys or more for each wave.  One decode row at
-// 32/8 heads of 128 with 128, 256, 384 and 512 workgroups in all: 15001 keys 15.7, 12.5, 18.3, 16.8 us;
-// 120001 keys 64, 42, 52, 47 (two of them stand on a CU, but 384 leave half with one).
+// workgroups as there are CUs, one group of keys or more for each wave.  With 128, 256, 384 and
+// 512 workgroups in all, us: one row at 32/8 heads of 128 of 15001 keys 11.8, 10.0, 14.4, 13.5, of
+// 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23 (one stands on a CU at a time).
 constexpr long kTilesFrom = 240, kSharers = 256;
 
-Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
+Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
     const long R = (long)T * (n_heads / n_kv);
     p.blocks = (int)((R + kTileRows - 1) / kTileRows);
@@ -1142,6 +1317,7 @@ Kv4Plan kv4_plan(int n_heads, int n_kv, int T, int ctx_len) {
         return p;
     }
     p.blocks = (int)((R + 15) / 16);
+    p.few = R <= 16 / (d_head / 32);
     const long groups = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
     p.nch = (int)std::max(1l, std::min((groups + kWaves - 1) / kWaves, kSharers / ((long)p.blocks * n_kv)));
     return p;
@@ -1152,7 +1328,7 @@ static_assert(kSharers <= kSmallMaxTiles, "a counter for each block whose keys a
 
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1) return 0;   // refused by the launch
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
     return p.nch > 1 ? (size_t)T * n_heads * p.nch * kv4_part(d_head) * sizeof(float) : 0;
 }
 
@@ -1164,7 +1340,7 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
            ctx_len, max_seq);
     VH_ARG((long)T * n_heads < (1l << 31), "attn: %d rows of %d heads", T, n_heads);
     VH_ARG(!m || (m->ld >= n_heads * d_head && (!m->pos_dev || T == 1)), "attn: bad model call");
-    const Kv4Plan p = kv4_plan(n_heads, n_kv, T, ctx_len);
+    const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
     VH_ARG(p.blocks <= 65535 && n_kv <= 65535 && (size_t)T * n_heads / n_kv * (n_heads / n_kv) < (1ull << 32),
            "attn: %d rows of %d heads over %d KV heads are beyond a launch", T, n_heads, n_kv);
     VH_ARG(p.nch == 1 || (part && attn_kv4_part_bytes(n_heads, n_kv, d_head, T, ctx_len) < (1ull << 31)), "attn: no scratch");
@@ -1202,8 +1378,15 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
         return VLRF_HIP_OK;
     }
     const dim3 grid(p.nch, n_kv, p.blocks);
-    if (d_head == 64) VH_LAUNCH(kv4_attn_rows_kernel<64>, grid, dim3(64 * kWaves), 0, s, a);
-    else VH_LAUNCH(kv4_attn_rows_kernel<128>, grid, dim3(64 * kWaves), 0, s, a);
+#define VH_ROWS(D, FEW) VH_LAUNCH((kv4_attn_rows_kernel<D, FEW>), grid, dim3(64 * kWaves), 0, s, a)
+    if (p.few) {
+        if (d_head == 64) VH_ROWS(64, true);
+        else VH_ROWS(128, true);
+    } else {
+        if (d_head == 64) VH_ROWS(64, false);
+        else VH_ROWS(128, false);
+    }
+#undef VH_ROWS
     VH_LAUNCHED();
     if (p.nch == 1 || merged) return VLRF_HIP_OK;
     if (d_head == 64) VH_LAUNCH(kv4_merge_kernel<64>, dim3(T * n_heads), dim3(512), 0, s, part, p.nch, out, a.out16);
