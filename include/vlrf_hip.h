@@ -135,6 +135,8 @@ int vlrf_hip_kv_dequant(vlrf_hip_kv_t kv, int layer, int ctx_len, float* K_out, 
  * d_head 64, ctx_len <= 8192 and less than 8 MiB of K/V one launch (each head's
  * context in at most 16 chunks, merged by the head's last workgroup), else one
  * that reads K/V once per four query heads and, over more than one chunk, a merge.
+ * A Q4_0 cache at any length: one launch, K/V read once (vlrf_hip_attn_chunk's), and
+ * a merge where more than 32 workgroups share the keys of a KV head.
  * Replaces the decode branch of AttentionBlock::forward: dequant_into +
  * reshape/expand_kv_heads + sdp_heads (attention.hpp:127-176). */
 int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out,
@@ -262,8 +264,8 @@ int vlrf_synth_normal(uint64_t seed, uint64_t stream, float std_dev, float* out,
 int vlrf_synth_tokens(uint64_t seed, uint64_t stream, int vocab, int32_t* out, int64_t n);
 
 /* ============================================================================
- * Decoder model (Llama-style: RMSNorm, RoPE half-split, SwiGLU, GQA; F32, F16
- * or Q8_0 KV cache).
+ * Decoder model (Llama-style: RMSNorm, RoPE half-split, SwiGLU, GQA; F32, F16,
+ * Q8_0 or Q4_0 KV cache).
  * Replaces the decode hot loop of TransformerModel::forward/generate
  * (transformer.hpp:335-424, 439-547) with a device-resident step: only token
  * ids cross PCIe.
@@ -273,7 +275,7 @@ typedef struct vlrf_hip_model_config {
     float   norm_eps, rope_theta;
     int32_t weight_dtype;   /* VLRF_HIP_DT_Q8_0 / VLRF_HIP_DT_Q4_0 / VLRF_HIP_DT_F32 for the projections */
     int32_t kv_dtype;       /* VLRF_HIP_KV_F32 / _F16 / _Q8_0: ModelConfig::kv_cache_dtype (config.hpp),
-                               the reference's KVCacheDType numbering, whose default F32 is 0 */
+                               the reference's KVCacheDType numbering, whose default F32 is 0; or _Q4_0 */
 } vlrf_hip_model_config;
 
 int  vlrf_hip_model_create(vlrf_hip_ctx_t ctx, const vlrf_hip_model_config* cfg,

@@ -129,7 +129,8 @@ def test_append_of_no_numbers(ctx):
     (4, 1, 64, 1, 0.125), (4, 4, 64, 2, 0.125), (32, 4, 64, 31, 0.125), (32, 4, 64, 32, 0.125), (8, 8, 128, 33, 0.1),
     (32, 8, 128, 127, 0.1), (32, 8, 128, 128, 0.1), (32, 4, 64, 129, 0.125), (24, 8, 64, 500, 0.125), (28, 4, 128, 777, 0.1),
     (16, 1, 64, 1000, 0.125), (17, 1, 128, 333, 0.1), (40, 1, 64, 2049, 0.125), (32, 8, 128, 4097, -0.1), (32, 4, 64, 4096, 0.0),
-    (6, 2, 64, 9001, 0.125), (32, 8, 128, 6001, 1.5), (4, 1, 64, 40011, 0.125)])
+    (6, 2, 64, 9001, 0.125), (32, 8, 128, 6001, 1.5), (4, 1, 64, 40011, 0.125),
+    (256, 256, 64, 100, 0.125), (250, 250, 128, 300, 0.1)])
 def test_decode_attention(ctx, H, G, d, n, scale):
     """All group sizes, edges of the groups of keys; rows behind the context hold NaN; the call that
     allocates nothing gives the same bits, and so does a second call."""
@@ -166,7 +167,8 @@ def test_decode_attention(ctx, H, G, d, n, scale):
     (24, 8, 64, 7, 33, 0.125), (28, 4, 128, 11, 40, 0.1), (32, 4, 64, 33, 33, 0.125), (32, 4, 64, 32, 64, -0.125),
     (8, 2, 128, 64, 64, 0.1), (16, 8, 64, 65, 200, 0.125), (17, 1, 64, 31, 95, 0.125), (32, 8, 128, 100, 1000, 0.1),
     (4, 4, 128, 257, 300, 0.1), (8, 2, 64, 300, 1029, 0.125), (4, 1, 64, 700, 700, 0.125), (12, 4, 128, 129, 3001, 0.1),
-    (32, 8, 128, 1, 5000, 0.1), (32, 4, 64, 3, 9000, 0.125), (8, 8, 128, 513, 513, 2.0), (2, 1, 128, 1500, 1500, 0.1)])
+    (32, 8, 128, 1, 5000, 0.1), (32, 4, 64, 3, 9000, 0.125), (8, 8, 128, 513, 513, 2.0), (2, 1, 128, 1500, 1500, 0.1),
+    (256, 256, 64, 3, 100, 0.125), (128, 128, 64, 129, 200, 0.125), (128, 128, 64, 127, 200, 0.125), (4, 4, 128, 4, 300, 0.1)])
 def test_chunk_attention(ctx, H, G, d, T, n, scale):
     """Chunks from one row on: ragged ones, groups of keys on the diagonal, few rows behind many keys."""
     print(f"[case] kv4 chunk H={H} G={G} d={d} T={T} n={n} scale={scale}", flush=True)
@@ -430,6 +432,10 @@ def test_refusals(ctx):
         return lib.vlrf_hip_attn_chunk(h, layer, q, o, heads, T, n, C.c_float(0.1))
 
     assert chunk() == 0
+    for o in (out.ptr, out.ptr + 4, out.ptr + 3 * 4 * 64 * 4 - 4):   # q and out side by side, not over each other
+        assert chunk(q=out.ptr, o=o) == _lib.ERR_ARG and "overlap" in _lib.last_error()
+        assert chunk(q=o, o=out.ptr) == _lib.ERR_ARG
+    assert chunk(q=x.ptr, o=x.ptr + 3 * 4 * 64 * 4) == 0
     for bad in (dict(layer=1), dict(layer=-1), dict(q=None), dict(o=None), dict(o=x.ptr), dict(heads=3), dict(heads=0),
                 dict(heads=-2), dict(T=0), dict(T=31), dict(T=-1), dict(n=51), dict(n=0), dict(n=2), dict(n=-5)):
         assert chunk(**bad) == _lib.ERR_ARG, bad

@@ -100,7 +100,8 @@ def _models(ctx, cfg, seed):
 
 @pytest.mark.parametrize("n_heads,n_kv,d_model,cap,tokens,weights", [
     (4, 1, 256, 160, 40, V.DT_Q8_0), (4, 4, 256, 64, 40, V.DT_Q4_0), (8, 2, 1024, 300, 40, V.DT_Q8_0),
-    (8, 8, 512, 1100, 300, V.DT_Q8_0), (8, 1, 1024, 700, 300, V.DT_Q4_0), (4, 2, 256, 80, 20, V.DT_F32)])
+    (8, 8, 512, 1100, 300, V.DT_Q8_0), (8, 1, 1024, 700, 300, V.DT_Q4_0), (4, 2, 256, 80, 20, V.DT_F32),
+    (4, 1, 256, 70000, 10, V.DT_Q8_0)])
 def test_steps(ctx, n_heads, n_kv, d_model, cap, tokens, weights):
     """Logits of teacher-forced steps, and the rows they store, against the layers attending to what the cache
     holds (f32-class: 1e-3 of the largest). Not to blocks of the reference's own: a value within f32 rounding

@@ -628,9 +628,11 @@ int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out,
     VH_ARG(layer >= 0 && layer < kv->n_layers, "attn_chunk: layer %d out of range", layer);
     VH_ARG(kv->layers[layer].dtype == VLRF_HIP_KV_Q4_0, "attn_chunk: the cache is not Q4_0 (dtype %d)",
            kv->layers[layer].dtype);
-    VH_ARG(q && out && q != out, "attn_chunk: null or shared pointer");
+    VH_ARG(q && out, "attn_chunk: null pointer");
     VH_ARG(T >= 1 && T <= ctx_len && ctx_len <= kv->max_seq, "attn_chunk: %d rows of %d keys in a cache of %d", T, ctx_len,
            kv->max_seq);
+    const uintptr_t from = (uintptr_t)q, to = (uintptr_t)out, bytes = (uintptr_t)T * std::max(n_heads, 0) * kv->d_head * sizeof(float);
+    VH_ARG(to >= from + bytes || from >= to + bytes, "attn_chunk: q and out overlap");
     return attn_kv4(kv, layer, q, out, n_heads, T, ctx_len, scale);
 }
 

@@ -43,12 +43,12 @@ __device__ __forceinline__ float kv4_inverse(uint32_t d16) {
 // Appending.  A workgroup takes CB blocks of 32 elements of one head's K or V rows at a
 // group of 32 key positions, a thread eight elements of a row (the heads of a group
 // follow each other, so that whole rows are read at a time: 16000 rows of 8 heads of
-// 128 52 us, with the groups of a head side by side 55.5):
+// 128 29 us, with the groups of a head side by side 32):
 // the four lanes of a block find its extreme by quad exchanges, and each has a word of
 // codes.  K's words go out as they are, a row's side by side.  V's bytes and the scales
 // are turned in LDS, where a whole group's are side by side, and go out in words; of a
 // group that the rows fill in part, byte by byte, so that the others stay.
-// Bound by the rows' bytes: that is 280 MB at 5.4 TB/s.  One row takes the time of the call.
+// Bound by the rows' bytes: that is 149 MB at 5.1 TB/s.  One row takes the time of the call.
 struct Kv4Append {
     const float *k, *v;       // [T][ld]
     uint8_t *kc, *vc;
@@ -1312,13 +1312,14 @@ struct Kv4Plan {
 // workgroups as there are CUs, one group of keys or more for each wave.  With 128, 256, 384 and
 // 512 workgroups in all, us: one row at 32/8 heads of 128 of 15001 keys 11.8, 10.0, 14.4, 13.5, of
 // 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23 (one stands on a CU at a time).
+// With less than a tile of rows a KV head most of the many rows would be none.
 constexpr long kTilesFrom = 240, kSharers = 256;
 
 Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
     const long R = (long)T * (n_heads / n_kv);
     p.blocks = (int)((R + kTileRows - 1) / kTileRows);
-    if ((long)p.blocks * n_kv >= kTilesFrom) {
+    if (T > 1 && R >= kTileRows && (long)p.blocks * n_kv >= kTilesFrom) {
         p.tiles = true;
         return p;
     }
