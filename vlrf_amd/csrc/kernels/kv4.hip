@@ -989,6 +989,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
 // a quarter of the conversions, which cost more (16 cycles a weight and block).  Stages
 // with a larger scale, or one that is no number, come last, with codes and scales apart.
 // Each wave keeps its rows to the end, so nothing is merged.  Three passes, as above.
+// 1777 rows of 4001 keys at 32/8 heads of 128 226 us: 0.40 PFLOP/s of the attention's own
+// 91 GFLOP, 1.0 of the f16 products (two for a score, three for an output) where a
+// large product alone reaches 1.18.  A third product for the scores in place of the scaling
+// (K whole, in two pieces) took as long, one product for each took 28 % less.
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 
 template <int NB>
