@@ -130,7 +130,8 @@ def test_append_of_no_numbers(ctx):
     (32, 8, 128, 127, 0.1), (32, 8, 128, 128, 0.1), (32, 4, 64, 129, 0.125), (24, 8, 64, 500, 0.125), (28, 4, 128, 777, 0.1),
     (16, 1, 64, 1000, 0.125), (17, 1, 128, 333, 0.1), (40, 1, 64, 2049, 0.125), (32, 8, 128, 4097, -0.1), (32, 4, 64, 4096, 0.0),
     (6, 2, 64, 9001, 0.125), (32, 8, 128, 6001, 1.5), (4, 1, 64, 40011, 0.125),
-    (256, 256, 64, 100, 0.125), (250, 250, 128, 300, 0.1)])
+    (256, 256, 64, 100, 0.125), (250, 250, 128, 300, 0.1),
+    (64, 1, 128, 40001, 0.1), (24, 1, 64, 40001, 0.125)])
 def test_decode_attention(ctx, H, G, d, n, scale):
     """All group sizes, edges of the groups of keys; rows behind the context hold NaN; the call that
     allocates nothing gives the same bits, and so does a second call."""
@@ -168,7 +169,8 @@ def test_decode_attention(ctx, H, G, d, n, scale):
     (8, 2, 128, 64, 64, 0.1), (16, 8, 64, 65, 200, 0.125), (17, 1, 64, 31, 95, 0.125), (32, 8, 128, 100, 1000, 0.1),
     (4, 4, 128, 257, 300, 0.1), (8, 2, 64, 300, 1029, 0.125), (4, 1, 64, 700, 700, 0.125), (12, 4, 128, 129, 3001, 0.1),
     (32, 8, 128, 1, 5000, 0.1), (32, 4, 64, 3, 9000, 0.125), (8, 8, 128, 513, 513, 2.0), (2, 1, 128, 1500, 1500, 0.1),
-    (256, 256, 64, 3, 100, 0.125), (128, 128, 64, 129, 200, 0.125), (128, 128, 64, 127, 200, 0.125), (4, 4, 128, 4, 300, 0.1)])
+    (256, 256, 64, 3, 100, 0.125), (128, 128, 64, 129, 200, 0.125), (128, 128, 64, 127, 200, 0.125), (4, 4, 128, 4, 300, 0.1),
+    (32, 8, 128, 13, 3001, 0.1), (16, 1, 64, 21, 12001, 0.125), (32, 8, 128, 5, 6001, 0.1), (32, 8, 128, 33, 700, 0.1)])
 def test_chunk_attention(ctx, H, G, d, T, n, scale):
     """Chunks from one row on: ragged ones, groups of keys on the diagonal, few rows behind many keys."""
     print(f"[case] kv4 chunk H={H} G={G} d={d} T={T} n={n} scale={scale}", flush=True)
@@ -183,7 +185,8 @@ def test_chunk_attention(ctx, H, G, d, T, n, scale):
     assert (err <= bound).all() and (got[-5:] == 7).all()
 
 
-@pytest.mark.parametrize("H,G,d,T,n", [(8, 2, 64, 40, 100), (4, 1, 128, 150, 150), (8, 2, 128, 300, 400), (2, 2, 64, 3, 70)])
+@pytest.mark.parametrize("H,G,d,T,n", [(8, 2, 64, 40, 100), (4, 1, 128, 150, 150), (8, 2, 128, 300, 400), (2, 2, 64, 3, 70),
+                                         (8, 2, 64, 600, 700)])
 def test_chunk_attention_masked_no_numbers(ctx, H, G, d, T, n):
     """A key or a value that is no number reaches the rows that see it and no other: the others
     are as far from the 64-bit result as they may be without it."""

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // ---- attention --------------------------------------------------------------------
 // The T * rep query rows of a KV head (rep query heads share it) stand as rows t rep
 // + r.  For few of them a workgroup takes 16, and where blocks of 16 are few several
-// share a block's keys: the eight waves of each take groups of 32 keys in turn, each
+// share a block's keys (for the fewest, as said at "few rows", 16 / NB): the eight waves of each take groups of 32 keys in turn, each
 // with its own running maximum and sum, and merge through LDS, and the workgroup that
 // comes last merges all of a block's.
 // One decode row at 32/8 heads of 128: 120001 keys 34.5 us (138 MB, 4.0 TB/s, what a large
@@ -661,8 +661,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(const float* part)
 constexpr int kMergedChunks = 32;
 
 // ---- few rows ---------------------------------------------------------------------
-// Where a KV head's rows are 16 / NB or fewer (a decode step of a usual group) the 16
-// columns stand for its rows and blocks: column NB row + b has the row's q where its block
+// In a block of 16 / NB rows (a decode step of a usual group) the 16 columns stand for
+// its rows and a head's blocks: column NB row + b has the row's q where its block
 // is b, zeros elsewhere, and the weights times b's scales of V.  So a lane loads, splits and
 // scales one block of q and of the scales instead of all, which is most of the work of a
 // group of keys; the columns' scores of a row are summed by exchanges within four lanes,
@@ -1317,7 +1317,13 @@ struct Kv4Plan {
 // 512 workgroups in all, us: one row at 32/8 heads of 128 of 15001 keys 11.8, 10.0, 14.4, 13.5, of
 // 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23 (one stands on a CU at a time).
 // With less than a tile of rows a KV head most of the many rows would be none.
-constexpr long kTilesFrom = 240, kSharers = 256;
+// Blocks of few rows, whose groups of keys cost less but are read once more for each, where
+// that is one block or all of them stand on the CUs at once with up to four groups a wave.  With 16
+// rows / few, us, at 32/8 heads of 128: 5 rows of 3000 keys (2 groups) 10.1 / 8.4, of 6000 (4)
+// 12.3 / 11.6, 8 of 3000 (3) 10.9 / 10.1, of 6000 (6) 12.4 / 14.7, 21 of 700 (3) 9.8 / 8.2, of 1500
+// (6) 11.6 / 12.6, 48 of 250 (384 blocks) 7.0 / 8.5; at 32/4 of 64: 64 of 700 (3) 8.7 / 6.7,
+// 233 of 700 (932 blocks) 10.4 / 14.4.
+constexpr long kTilesFrom = 240, kSharers = 256, kFewGroups = 4;
 
 Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
@@ -1327,10 +1333,16 @@ Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
         p.tiles = true;
         return p;
     }
-    p.blocks = (int)((R + 15) / 16);
-    p.few = R <= 16 / (d_head / 32);
     const long groups = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
-    p.nch = (int)std::max(1l, std::min((groups + kWaves - 1) / kWaves, kSharers / ((long)p.blocks * n_kv)));
+    auto blocks_of = [&](int rows) {
+        p.blocks = (int)((R + rows - 1) / rows);
+        p.nch = (int)std::max(1l, std::min((groups + kWaves - 1) / kWaves, kSharers / ((long)p.blocks * n_kv)));
+        return (groups + (long)p.nch * kWaves - 1) / ((long)p.nch * kWaves);   // groups of keys of a wave
+    };
+    const int fewest = 16 / (d_head / 32);
+    const long each = blocks_of(fewest);
+    p.few = R <= fewest || ((long)p.blocks * n_kv <= kSharers && each <= kFewGroups);
+    if (!p.few) blocks_of(16);
     return p;
 }
 
