@@ -90,7 +90,7 @@ class Decoder:
 
 def _cfg(n_heads, n_kv, d_model, cap, n_layers=2, weight_dtype=V.DT_Q8_0):
     return dict(F.tiny(weight_dtype, n_layers=n_layers, max_seq_len=cap), n_heads=n_heads, n_kv_heads=n_kv,
-                d_model=d_model, d_ff=2 * d_model, kv_dtype=V.KV_Q4_0)
+                d_model=d_model, d_ff=2 * d_model if d_model <= 1024 else 512, kv_dtype=V.KV_Q4_0)
 
 
 def _models(ctx, cfg, seed):
@@ -148,7 +148,7 @@ def test_generation_is_the_steps(ctx, monkeypatch, n_heads, n_kv, d_model, cap):
 
 @pytest.mark.parametrize("n_heads,n_kv,d_model,chunks", [
     (4, 1, 256, (70, 45)), (8, 2, 1024, (1, 33, 90)), (8, 8, 512, (300, 20)), (8, 8, 512, (3900, 200)),
-    (16, 2, 1024, (600,))])
+    (16, 2, 1024, (600,)), (32, 8, 2048, (1700,)), (32, 8, 4096, (900, 30))])
 def test_prefill_layer(ctx, n_heads, n_kv, d_model, chunks):
     """One layer over embedded rows in chunks (few rows, and enough for the many-rows kernel): the output
     in the bf16 class (1e-2) of the layer attending to what the cache holds, whose values are within half

@@ -1309,28 +1309,42 @@ struct Kv4Plan {
     int blocks = 1, nch = 1;                 // blocks of rows of a KV head, workgroups that share a block's keys
 };
 
-// The kernel for many rows wins once its workgroups fill the CUs (rows kernel's / tiles kernel's
-// time): 1777 rows of 4001 keys at 32/8 heads of 128 (448 workgroups) 406 / 228 us, 1024 of 1024
-// (256) 76 / 60, 1024 of 2048 at 32/4 of 64 (256) 64 / 63; but 700 of 4000 (176) 197 / 206, 512 of
-// 1024 (128) 46 / 57.  Below, blocks of 16 rows, whose keys are shared out to as many
-// workgroups as there are CUs, one group of keys or more for each wave.  With 128, 256, 384 and
-// 512 workgroups in all, us: one row at 32/8 heads of 128 of 15001 keys 11.8, 10.0, 14.4, 13.5, of
-// 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23 (one stands on a CU at a time).
-// With less than a tile of rows a KV head most of the many rows would be none.
+// Tiles or blocks of 16 rows: whichever is estimated to take less.  A block of 16 rows costs a
+// fixed time and each of its rows' keys another; tiles that stand alone on a CU take a time a key of the
+// longest row, where some share one a little more, and where there are many the CUs are evenly
+// full.  In us, fitted to 206 pairs of times (T 200 to 6400, contexts from T to T + 6000, 11 layouts): the
+// choice costs 0.1 % on average and 10 % at most, where a limit on the number of tiles cost 2 %
+// and 43 % (a prompt of 3700 tokens at 8/8 heads of 128: 140 in blocks, 176 in 232 tiles, of which the
+// longest take all the time; 900 of 4900 at 32/8, as many: 282 and 234).
+// In blocks, the keys are shared out to as many workgroups as there are CUs, one group of keys
+// or more for each wave.  With 128, 256, 384 and 512 workgroups in all, us: one row at 32/8 heads of 128
+// of 15001 keys 11.8, 10.0, 14.4, 13.5, of 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23
+// (one stands on a CU at a time).
 // Blocks of few rows, whose groups of keys cost less but are read once more for each, where
 // that is one block or all of them stand on the CUs at once with up to four groups a wave.  With 16
 // rows / few, us, at 32/8 heads of 128: 5 rows of 3000 keys (2 groups) 10.1 / 8.4, of 6000 (4)
 // 12.3 / 11.6, 8 of 3000 (3) 10.9 / 10.1, of 6000 (6) 12.4 / 14.7, 21 of 700 (3) 9.8 / 8.2, of 1500
 // (6) 11.6 / 12.6, 48 of 250 (384 blocks) 7.0 / 8.5; at 32/4 of 64: 64 of 700 (3) 8.7 / 6.7,
 // 233 of 700 (932 blocks) 10.4 / 14.4.
-constexpr long kTilesFrom = 240, kSharers = 256, kFewGroups = 4;
+constexpr long kSharers = 256, kFewGroups = 4;
+
+struct Kv4Cost {
+    double block, pairs;             // a workgroup of 16 rows, a million keys of a row
+    double start, alone, beside;     // tiles: fixed, a key of the longest row with up to 256 tiles, with more
+    double full;                     // 32768 keys of a row (a key of a tile on every CU)
+};
+constexpr Kv4Cost kCost64 = {0.0071, 0.80, 3.3, 0.026, 0.030, 0.025}, kCost128 = {0.0195, 1.80, 5.0, 0.0465, 0.055, 0.041};
 
 Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
-    const long R = (long)T * (n_heads / n_kv);
-    p.blocks = (int)((R + kTileRows - 1) / kTileRows);
-    if (T > 1 && R >= kTileRows && (long)p.blocks * n_kv >= kTilesFrom) {
+    const long R = (long)T * (n_heads / n_kv), tiles = (R + kTileRows - 1) / kTileRows * n_kv;
+    const Kv4Cost& c = d_head == 64 ? kCost64 : kCost128;
+    const double pairs = (double)n_heads * T * (ctx_len - 0.5 * (T - 1));
+    const double in_blocks = c.block * (double)((R + 15) / 16 * n_kv) + c.pairs * 1e-6 * pairs;
+    const double in_tiles = c.start + std::max(ctx_len * (tiles <= 256 ? c.alone : c.beside), c.full * pairs / 32768);
+    if (T > 1 && R >= kTileRows && in_tiles < in_blocks) {   // a tile of rows at least: less is mostly none
         p.tiles = true;
+        p.blocks = (int)((R + kTileRows - 1) / kTileRows);
         return p;
     }
     const long groups = (ctx_len + kv4::kKeys - 1) / kv4::kKeys;
