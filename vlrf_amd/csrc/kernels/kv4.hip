@@ -1312,7 +1312,7 @@ struct Kv4Plan {
 // Tiles or blocks of 16 rows: whichever is estimated to take less.  A block of 16 rows costs a
 // fixed time and each of its rows' keys another; tiles that stand alone on a CU take a time a key of the
 // longest row, where some share one a little more, and where there are many the CUs are evenly
-// full.  In us, fitted to 206 pairs of times (T 200 to 6400, contexts from T to T + 6000, 11 layouts): the
+// full.  In us, fitted to 362 pairs of times (T 200 to 6400, contexts from T to T + 6000, 11 layouts): the
 // choice costs 0.1 % on average and 10 % at most, where a limit on the number of tiles cost 2 %
 // and 43 % (a prompt of 3700 tokens at 8/8 heads of 128: 140 in blocks, 176 in 232 tiles, of which the
 // longest take all the time; 900 of 4900 at 32/8, as many: 282 and 234).
