@@ -171,7 +171,7 @@ def test_decode_attention(ctx, H, G, d, n, scale):
     (32, 8, 128, 1, 5000, 0.1), (32, 4, 64, 3, 9000, 0.125), (8, 8, 128, 513, 513, 2.0), (2, 1, 128, 1500, 1500, 0.1),
     (256, 256, 64, 3, 100, 0.125), (128, 128, 64, 129, 200, 0.125), (128, 128, 64, 127, 200, 0.125), (4, 4, 128, 4, 300, 0.1),
     (32, 8, 128, 13, 3001, 0.1), (16, 1, 64, 21, 12001, 0.125), (32, 8, 128, 5, 6001, 0.1), (32, 8, 128, 33, 700, 0.1),
-    (128, 128, 64, 200, 333, 0.125), (128, 64, 128, 150, 333, -0.1), (64, 64, 128, 300, 301, 0.1)])
+    (128, 128, 64, 200, 333, 0.125), (128, 64, 128, 150, 333, -0.1), (256, 64, 128, 150, 333, -0.1), (64, 64, 128, 300, 301, 0.1)])
 def test_chunk_attention(ctx, H, G, d, T, n, scale):
     """Chunks from one row on: ragged ones, groups of keys on the diagonal, few rows behind many keys."""
     print(f"[case] kv4 chunk H={H} G={G} d={d} T={T} n={n} scale={scale}", flush=True)
@@ -187,7 +187,7 @@ def test_chunk_attention(ctx, H, G, d, T, n, scale):
 
 
 @pytest.mark.parametrize("H,G,d,T,n", [(8, 2, 64, 40, 100), (4, 1, 128, 150, 150), (8, 2, 128, 300, 400), (2, 2, 64, 3, 70),
-                                         (8, 2, 64, 600, 700), (128, 128, 64, 200, 333), (128, 64, 128, 150, 333)])
+                                         (8, 2, 64, 600, 700), (128, 128, 64, 200, 333), (128, 64, 128, 150, 333), (256, 64, 128, 150, 333)])
 def test_chunk_attention_masked_no_numbers(ctx, H, G, d, T, n):
     """A key or a value that is no number reaches the rows that see it and no other: the others
     are as far from the 64-bit result as they may be without it."""
@@ -215,7 +215,7 @@ def test_chunk_attention_masked_no_numbers(ctx, H, G, d, T, n):
     assert np.isnan(got["first"]).all()
 
 
-@pytest.mark.parametrize("H,G,T", [(8, 2, 1), (8, 2, 3), (8, 2, 200), (128, 64, 150)])
+@pytest.mark.parametrize("H,G,T", [(8, 2, 1), (8, 2, 3), (8, 2, 200), (128, 64, 150), (256, 64, 150)])
 @pytest.mark.parametrize("k_std,v_std", [(1.0, 5e4), (300.0, 1.0), (1.0, 1e-4), (1e-3, 30.0), (2e4, 2e4)])
 def test_ranges_of_the_cache(ctx, k_std, v_std, H, G, T):
     """Scales up to f16's largest and small ones, side by side in one group of keys."""

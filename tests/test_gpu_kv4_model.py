@@ -148,7 +148,7 @@ def test_generation_is_the_steps(ctx, monkeypatch, n_heads, n_kv, d_model, cap):
 
 @pytest.mark.parametrize("n_heads,n_kv,d_model,chunks", [
     (4, 1, 256, (70, 45)), (8, 2, 1024, (1, 33, 90)), (8, 8, 512, (300, 20)), (8, 8, 512, (3900, 200)),
-    (16, 2, 1024, (600,)), (32, 8, 2048, (1700,)), (32, 8, 4096, (900, 30))])
+    (16, 2, 1024, (600,)), (32, 8, 2048, (1700,)), (32, 8, 4096, (1777, 30))])
 def test_prefill_layer(ctx, n_heads, n_kv, d_model, chunks):
     """One layer over embedded rows in chunks (few rows, and enough for the many-rows kernel): the output
     in the bf16 class (1e-2) of the layer attending to what the cache holds, whose values are within half

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // ---- attention --------------------------------------------------------------------
 // The T * rep query rows of a KV head (rep query heads share it) stand as rows t rep
 // + r.  For few of them a workgroup takes 16, and where blocks of 16 are few several
-// share a block's keys (for the fewest, as said at "few rows", 16 / NB): the eight waves of each take groups of 32 keys in turn, each
+// share a block's keys (for the fewest, as said at "few rows", 16 / NB): the eight (or four) waves of each take groups of 32 keys in turn, each
 // with its own running maximum and sum, and merge through LDS, and the workgroup that
 // comes last merges all of a block's.
 // One decode row at 32/8 heads of 128: 120001 keys 34.5 us (138 MB, 4.0 TB/s, what a large
@@ -789,18 +789,18 @@ __device__ __forceinline__ void kv4_few_keys(Kv4Few<NB>& r, const Kv4Raw<NB, 1>&
     }
 }
 
-constexpr int kWaves = 8;   // of a workgroup of 16 rows
+constexpr int kWaves = 8;   // of a workgroup that has a CU to itself; half of them where two share it
 
-template <int D, int ROWS>
+template <int D, int ROWS, int W>
 struct Kv4WavesLds {
-    float o[kWaves][ROWS * (D + 4)], m[ROWS][kWaves], l[ROWS][kWaves];
+    float o[W][ROWS * (D + 4)], m[ROWS][W], l[ROWS][W];
 };
 
-template <int D, bool FEW>
-__global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
+template <int D, bool FEW, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
     constexpr int NB = D / 32, ROWS = FEW ? 16 / NB : 16, OS = D + 4;
     __shared__ int last;
-    __shared__ __align__(16) Kv4WavesLds<D, ROWS> x;
+    __shared__ __align__(16) Kv4WavesLds<D, ROWS, W> x;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, L = lane >> 4;
     const int lane_row = FEW ? c / NB : c, own = FEW ? c % NB : 0;   // the lane's row, its block
     if (a.pos_dev) a.ctx = min(*a.pos_dev + 1, a.ctx);
@@ -809,8 +809,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     const uint16_t *ks = a.ks + g * a.scales, *vs = a.vs + g * a.scales;
     // Keys that the block's first and last row see.
     const int past = a.ctx - a.T + 1, fewest = past + kv4_token(a, row0), most = past + kv4_token(a, min(row0 + ROWS - 1, R - 1));
-    // The wave's groups of keys: every nch * kWaves-th, so that all share any context alike.
-    const int kb0 = chunk * kWaves + w, stride = nch * kWaves;
+    // The wave's groups of keys: every nch * W-th, so that all share any context alike.
+    const int kb0 = chunk * W + w, stride = nch * W;
     auto mine_of = [&](int groups) { return groups > kb0 ? (groups - kb0 + stride - 1) / stride : 0; };
     const int mine = mine_of((most + kv4::kKeys - 1) / kv4::kKeys), inside = min(mine, mine_of(fewest / kv4::kKeys));
 
@@ -896,13 +896,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     }
     __syncthreads();
     const int rows = min(ROWS, R - row0), tid = threadIdx.x;
-    for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
+    for (int i = tid; i < rows * (D / 4); i += 64 * W) {
         const int j = i / (D / 4), e = 4 * (i % (D / 4));
-        float m[kWaves], M = kNegInf, l = 0.f, v[4] = {};
+        float m[W], M = kNegInf, l = 0.f, v[4] = {};
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) M = fmaxf(M, m[k] = x.m[j][k]);
+        for (int k = 0; k < W; ++k) M = fmaxf(M, m[k] = x.m[j][k]);
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
+        for (int k = 0; k < W; ++k) {
             const float f = m[k] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[k] - M);
             const float4 y = *reinterpret_cast<const float4*>(&x.o[k][j * OS + e]);
             l = fmaf(f, x.l[j][k], l);
@@ -940,7 +940,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_attn_rows_kernel(Kv4Attn a
     constexpr int Q = D / 4, SHARES = 64 / Q, EACH = kMergedChunks / SHARES, PS = kv4_part(D);
     const auto pr = part_buffer(a.part);
     const int e = 4 * (lane % Q), share = lane / Q;
-    for (int j = w; j < rows; j += kWaves) {
+    for (int j = w; j < rows; j += W) {
         const size_t at = kv4_row(a, g, row0 + j);
         const int first = (int)(4 * at * nch * PS);
         const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, lane < nch ? first + 4 * (lane * PS + D) : kOutside, 0, 16));
@@ -1306,6 +1306,7 @@ namespace {
 struct Kv4Plan {
     bool tiles = false;                      // the kernel for many rows
     bool few = false;                        // the kernel for a column a row and block
+    int waves = kWaves;                      // of a block of 16 rows
     int blocks = 1, nch = 1;                 // blocks of rows of a KV head, workgroups that share a block's keys
 };
 
@@ -1313,9 +1314,9 @@ struct Kv4Plan {
 // fixed time and each of its rows' keys another; tiles that stand alone on a CU take a time a key of the
 // longest row, where some share one a little more, and where there are many the CUs are evenly
 // full.  In us, fitted to 362 pairs of times (T 200 to 6400, contexts from T to T + 6000, 11 layouts): the
-// choice costs 0.1 % on average and 10 % at most, where a limit on the number of tiles cost 2 %
-// and 43 % (a prompt of 3700 tokens at 8/8 heads of 128: 140 in blocks, 176 in 232 tiles, of which the
-// longest take all the time; 900 of 4900 at 32/8, as many: 282 and 234).
+// choice costs 0.1 % on average and 10 % at most, where a limit on the number of tiles cost 1 to
+// 3 % and 43 % (a prompt of 3700 tokens at 8/8 heads of 128: 119 in blocks, 176 in 232 tiles, of which
+// the longest take all the time; 900 of 4900 at 32/8, as many: 248 and 233).
 // In blocks, the keys are shared out to as many workgroups as there are CUs, one group of keys
 // or more for each wave.  With 128, 256, 384 and 512 workgroups in all, us: one row at 32/8 heads of 128
 // of 15001 keys 11.8, 10.0, 14.4, 13.5, of 120001 51, 34, 42, 39; 40 rows of 3001 keys 27, 16, 26, 23
@@ -1326,14 +1327,19 @@ struct Kv4Plan {
 // 12.3 / 11.6, 8 of 3000 (3) 10.9 / 10.1, of 6000 (6) 12.4 / 14.7, 21 of 700 (3) 9.8 / 8.2, of 1500
 // (6) 11.6 / 12.6, 48 of 250 (384 blocks) 7.0 / 8.5; at 32/4 of 64: 64 of 700 (3) 8.7 / 6.7,
 // 233 of 700 (932 blocks) 10.4 / 14.4.
-constexpr long kSharers = 256, kFewGroups = 4;
+// Where there are more blocks of 16 rows than CUs each has four waves instead of eight, and one
+// block's start and end run beside another's keys; at d_head 64 two of eight stand on a CU anyway, so
+// that only short contexts gain.  With 8 / 4 waves, us, at 32/8 heads of 128: 200 rows of 500 keys (400
+// blocks) 15.6 / 12.2, of 4200 66.5 / 63.6, 400 of 700 32.6 / 24.1, 100 of 1100 (200 blocks) 13.2 / 13.8; at
+// 32/4 of 64: 400 rows of 400 11.3 / 8.7, of 1400 24.7 / 23.8, of 4400 67.9 / 68.9.
+constexpr long kSharers = 256, kFewGroups = 4, kFourFrom64 = 2048;
 
 struct Kv4Cost {
     double block, pairs;             // a workgroup of 16 rows, a million keys of a row
     double start, alone, beside;     // tiles: fixed, a key of the longest row with up to 256 tiles, with more
     double full;                     // 32768 keys of a row (a key of a tile on every CU)
 };
-constexpr Kv4Cost kCost64 = {0.0071, 0.80, 3.3, 0.026, 0.030, 0.025}, kCost128 = {0.0195, 1.80, 5.0, 0.0465, 0.055, 0.041};
+constexpr Kv4Cost kCost64 = {0.0064, 0.86, 5.5, 0.027, 0.0305, 0.026}, kCost128 = {0.0115, 1.65, 8.7, 0.0455, 0.056, 0.042};
 
 Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     Kv4Plan p;
@@ -1356,7 +1362,10 @@ Kv4Plan kv4_plan(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
     const int fewest = 16 / (d_head / 32);
     const long each = blocks_of(fewest);
     p.few = R <= fewest || ((long)p.blocks * n_kv <= kSharers && each <= kFewGroups);
-    if (!p.few) blocks_of(16);
+    if (!p.few) {
+        blocks_of(16);
+        if ((long)p.blocks * n_kv > kSharers && (d_head == 128 || ctx_len <= kFourFrom64)) p.waves = kWaves / 2;
+    }
     return p;
 }
 
@@ -1415,13 +1424,16 @@ int launch_attn_kv4(hipStream_t s, const float* q, const KVLayer& L, int n_heads
         return VLRF_HIP_OK;
     }
     const dim3 grid(p.nch, n_kv, p.blocks);
-#define VH_ROWS(D, FEW) VH_LAUNCH((kv4_attn_rows_kernel<D, FEW>), grid, dim3(64 * kWaves), 0, s, a)
+#define VH_ROWS(D, FEW, W) VH_LAUNCH((kv4_attn_rows_kernel<D, FEW, W>), grid, dim3(64 * W), 0, s, a)
     if (p.few) {
-        if (d_head == 64) VH_ROWS(64, true);
-        else VH_ROWS(128, true);
+        if (d_head == 64) VH_ROWS(64, true, kWaves);
+        else VH_ROWS(128, true, kWaves);
+    } else if (p.waves == kWaves / 2) {
+        if (d_head == 64) VH_ROWS(64, false, kWaves / 2);
+        else VH_ROWS(128, false, kWaves / 2);
     } else {
-        if (d_head == 64) VH_ROWS(64, false);
-        else VH_ROWS(128, false);
+        if (d_head == 64) VH_ROWS(64, false, kWaves);
+        else VH_ROWS(128, false, kWaves);
     }
 #undef VH_ROWS
     VH_LAUNCHED();
