@@ -197,9 +197,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // ---- attention --------------------------------------------------------------------
 // The T * rep query rows of a KV head (rep query heads share it) stand as rows t rep
 // + r.  For few of them a workgroup takes 16, and where blocks of 16 are few several
-// share a block's keys (for the fewest, as said at "few rows", 16 / NB): the eight (or four) waves of each take groups of 32 keys in turn, each
-// with its own running maximum and sum, and merge through LDS, and the workgroup that
-// comes last merges all of a block's.
+// share a block's keys (for the fewest, as said at "few rows", 16 / NB): the eight or
+// four waves of each take groups of 32 keys in turn, each with its own running maximum
+// and sum, and merge through LDS, and the workgroup that comes last merges all of a
+// block's.
 // One decode row at 32/8 heads of 128: 120001 keys 34.5 us (138 MB, 4.0 TB/s, what a large
 // read reaches); 15001 keys 10.0 (17 MB, 1.7 TB/s) and 1500 keys 6.8, bound by the chain of
 // waits: the launch, the arguments, q and the keys, the group's products and weights, the waves'
