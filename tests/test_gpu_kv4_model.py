@@ -146,6 +146,17 @@ def test_generation_is_the_steps(ctx, monkeypatch, n_heads, n_kv, d_model, cap):
     assert kinds["attn"][1] >= 2 * cfg["n_layers"] * 3 and "qkv_attn" in kinds
 
 
+@pytest.mark.parametrize("n_heads,n_kv,d_model,cap,attn", [(4, 1, 256, 70000, 3), (8, 2, 1024, 300, 2)])
+def test_every_launch_of_a_step_is_timed(ctx, n_heads, n_kv, d_model, cap, attn):
+    """Append, attention and, where many workgroups share a KV head's keys, its merge; and what comes after."""
+    cfg = _cfg(n_heads, n_kv, d_model, cap, n_layers=4)
+    m = V.Model(ctx, cfg)
+    F.load_model(m, 76)
+    kinds = m.time_launches(5, 6)
+    calls = {k: v[1] for k, v in kinds.items()}
+    assert calls["attn"] == attn * 4 * 6 and calls["qkv_attn"] == calls["o_proj"] == calls["gate_up"] == calls["down"] == 4 * 6, calls
+
+
 @pytest.mark.parametrize("n_heads,n_kv,d_model,chunks", [
     (4, 1, 256, (70, 45)), (8, 2, 1024, (1, 33, 90)), (8, 8, 512, (300, 20)), (8, 8, 512, (3900, 200)),
     (16, 2, 1024, (600,)), (32, 8, 2048, (1700,)), (32, 8, 4096, (1777, 30))])

@@ -847,9 +847,9 @@ int vlrf_hip_model_time_launches(vlrf_hip_model_t m, int32_t first, int n_steps,
         calls[k] = 0;
     }
     hipStream_t s = m->ctx->stream;
-    // At most 6 launches per layer plus 3 per step (stand-alone attention with
-    // its combine, the embedding, the LM head and the argmax).
-    const int cap = n_steps * (6 * m->L + 3);
+    // At most 7 launches per layer plus 3 per step (stand-alone attention with
+    // its append and merge, the embedding, the LM head and the argmax).
+    const int cap = n_steps * (7 * m->L + 3);
     std::vector<hipEvent_t> ev(2 * (size_t)cap, nullptr);
     std::vector<int> kind(cap, 0);
     LaunchTimer t;
