@@ -454,3 +454,22 @@ def test_refusals(ctx):
     wide.append(0, x, x, 30)
     assert chunk(h=wide.h) == _lib.ERR_ARG and "d_head 96" in _lib.last_error()
     ctx.sync()
+
+
+@pytest.mark.parametrize("d", [32, 160, 256, 512, 544, 1024, 2048])
+def test_refused_d_head_of_attention(ctx, d):
+    """A cache of any whole number of blocks a row is appended to and read back; attention over it is an
+    error, whatever the size, by each of the three calls."""
+    print(f"[case] kv4 refused d_head={d}", flush=True)
+    H, G, n = 4, 1, 100
+    lib = V.lib()
+    kv = V.KVCache(ctx, 1, n, G, d, V.KV_Q4_0)
+    x = ctx.to_device(F.normal(100, "wide", n * d))
+    q, out = ctx.to_device(np.zeros(3 * H * d, np.float32)), ctx.to_device(np.full(3 * H * d, 7, np.float32))
+    kv.append(0, x, x, n)
+    for rc in (lib.vlrf_hip_attn_decode(kv.h, 0, q.ptr, out.ptr, H, n, C.c_float(0.1)),
+               lib.vlrf_hip_attn_decode_noalloc(kv.h, 0, q.ptr, out.ptr, H, n, C.c_float(0.1)),
+               lib.vlrf_hip_attn_chunk(kv.h, 0, q.ptr, out.ptr, H, 3, n, C.c_float(0.1))):
+        assert rc == _lib.ERR_ARG and f"d_head {d}" in _lib.last_error()
+    assert (out.download((3 * H * d,)) == 7).all()
+    assert np.array_equal(kv.read(0, 0, n)[1].ravel(), F.quantize(x.download((n, d)), V.DT_Q4_0))

@@ -5,6 +5,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -63,3 +64,22 @@ def test_null_handles_are_refused():
     assert lib.vlrf_hip_attn_chunk(None, 0, x, x, 1, 1, 1, 1.0) == _lib.ERR_ARG and "null cache" in _lib.last_error()
     h = C.c_void_p()
     assert lib.vlrf_hip_kv_create(None, 1, 1, 1, 64, V.KV_Q4_0, C.byref(h)) == _lib.ERR_ARG and h.value is None
+
+
+def test_scratch_of_refused_attention_is_none():
+    """The scratch of an attention is asked for before the launch refuses its sizes: none for those, any
+    d_head that a cache may have. In a process of its own: a division by no rows would end it."""
+    code = ("import sys; sys.path.insert(0, %r)\n"
+            "import ctypes as C\n"
+            "import vlrf_amd as V\n"
+            "part = V.lib()._ZN8vlrf_hip19attn_kv4_part_bytesEiiiii\n"
+            "part.restype, part.argtypes = C.c_size_t, [C.c_int] * 5\n"
+            "for d in (32, 96, 160, 256, 512, 544, 1024, 65536):\n"
+            "    for H, G, T, n in ((4, 1, 1, 100), (32, 8, 1, 120001), (32, 8, 40, 3001), (32, 8, 1777, 4001)):\n"
+            "        assert part(H, G, d, T, n) == 0, (H, G, d, T, n)\n"
+            "for H, G, T, n in ((0, 1, 1, 9000), (4, 0, 1, 9000), (4, 3, 1, 9000), (-4, 1, 1, 9000), (4, 1, 0, 9000), (4, 1, 9, 8)):\n"
+            "    assert part(H, G, 64, T, n) == 0, (H, G, T, n)\n"
+            "assert part(32, 8, 128, 1, 120001) == 32 * 32 * 132 * 4 and part(32, 4, 64, 1, 100) == 0\n"
+            "print('ok')" % ROOT)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", (r.returncode, r.stderr[-800:])

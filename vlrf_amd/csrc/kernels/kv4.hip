@@ -1374,7 +1374,8 @@ static_assert(kSharers <= kSmallMaxTiles, "a counter for each block whose keys a
 }  // namespace
 
 size_t attn_kv4_part_bytes(int n_heads, int n_kv, int d_head, int T, int ctx_len) {
-    if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1) return 0;   // refused by the launch
+    // Refused by the launch: no plan, and no scratch that would grow for such a call.
+    if (n_kv < 1 || n_heads < 1 || n_heads % n_kv || T < 1 || ctx_len < T || (d_head != 64 && d_head != 128)) return 0;
     const Kv4Plan p = kv4_plan(n_heads, n_kv, d_head, T, ctx_len);
     return p.nch > 1 ? (size_t)T * n_heads * p.nch * kv4_part(d_head) * sizeof(float) : 0;
 }
