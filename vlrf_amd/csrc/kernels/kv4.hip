@@ -213,8 +213,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 //            two), so p <= 2^14; rescaling O is rare and skipped by the wave.
 //   output   O^T = V^T P^T over the same codes: p times the key's scale, in two f16
 //            pieces, is the other operand.  It stays below 2^15 while scales are
-//            below 2; a block with a larger one among the 32 keys' has its products
-//            formed apart, scaled down by a power of two, and added scaled up.
+//            below 2.  Groups of 32 keys with a larger scale have their products formed
+//            apart, each row's times the power of two that brings the largest that
+//            the row sees to [2^14, 2^15), and added scaled back: no key's scale costs
+//            another's bits, and a key that the row does not see has no say.
 // A lane's scores are of the row that is its column in both products and of the keys
 // that its group of V's layout holds, so nothing moves between lanes but the
 // maximum's two exchanges a group.
@@ -387,16 +389,28 @@ __device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn&
     for (int i = 0; i < 2 * NB; ++i) r.o[n][i] = f4v{};
 }
 
-// How far a block's products are formed below: the exponent, over 2^0, of the largest finite
-// scale of V among the 32 keys.
-__device__ __forceinline__ int kv4_down(const uint4& vs) {
-    uint32_t top = 15;
+// A row's weights times a block's scales (vs) of 32 keys, formed apart: in two f16 pieces of
+// the products times 2^k, the largest of which over the keys lies in [2^14, 2^15); 2^-k is
+// returned.  end: as in kv4_weights; a key that the row does not see has no product, so
+// that neither its scale nor what it holds matters.  A product that is no number
+// stays one (the maximum passes over it).
+__device__ __forceinline__ float kv4_apart(const float (&p)[8], const uint4& vs, int end, h2v (&hi)[4], h2v (&lo)[4]) {
+    float w[8], top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t x = (word_of(vs, j >> 1) >> (16 * (j & 1) + 10)) & 31u;
-        top = x < 31u ? max(top, x) : top;
+    for (int e = 0; e < 8; ++e) {
+        const h2v d = as_h2(word_of(vs, e >> 1));
+        w[e] = kv4::key_of(0, e) >= end ? 0.f : p[e] * (float)((e & 1) ? d.y : d.x);
+        top = fmaxf(top, fabsf(w[e]));
     }
-    return (int)over_groups_max((float)top) - 15;
+    top = over_groups_max(top);
+    const int k = min(141 - (int)(__float_as_uint(top) >> 23), 126);
+    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand
+        const int e = 4 * (i >> 1) + (i & 1);
+        split2(w[e], up, w[e + 2], up, hi[i], lo[i]);
+    }
+    return __uint_as_float((uint32_t)(127 - k) << 23);
 }
 
 // KG groups of 32 keys from key0 on; src: their operands (k, v) and scales (ks, vs) by
@@ -532,41 +546,35 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
             h8v va, wa;   // even elements, odd elements
             src.v(kg, b, va, wa);
             const uint4 vs = src.vs(kg, b);
-            int down = 0;                                // powers of two that the block's products are formed below
-            if constexpr (MODE == kApart) down = kv4_down(vs);
-            const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
-                // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.  A key that the row
-                // does not see weighs 0 whatever its scale is.
                 h2v hi[4], lo[4];
+                float back = 1.f;
+                if constexpr (MODE == kApart) {
+                    static_assert(KG == 1, "weights of one group of keys");
+                    back = kv4_apart(s[n][0], vs, r.seen[n] - key0 - 4 * L, hi, lo);
+                } else {
+                    // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 4 * (i >> 1) + (i & 1);
-                    const h2v d0 = as_h2(word_of(vs, e >> 1)), d1 = as_h2(word_of(vs, (e >> 1) + 1));
-                    float f = (i & 1) ? d0.y : d0.x, g = (i & 1) ? d1.y : d1.x, p0 = s[n][kg][e], p1 = s[n][kg][e + 2];
-                    if constexpr (MODE == kApart) {
-                        f = 32 * kg + kv4::key_of(0, e) >= r.seen[n] - key0 - 4 * L ? 0.f : f;
-                        g = 32 * kg + kv4::key_of(0, e + 2) >= r.seen[n] - key0 - 4 * L ? 0.f : g;
-                        p0 *= scale_down;
-                        p1 *= scale_down;
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * (i >> 1) + (i & 1);
+                        const h2v d0 = as_h2(word_of(vs, e >> 1)), d1 = as_h2(word_of(vs, (e >> 1) + 1));
+                        split2(s[n][kg][e], (i & 1) ? d0.y : d0.x, s[n][kg][e + 2], (i & 1) ? d1.y : d1.x, hi[i], lo[i]);
                     }
-                    split2(p0, f, p1, g, hi[i], lo[i]);
                 }
                 const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
-                if (MODE != kApart || __builtin_amdgcn_readfirstlane(down) == 0) {
-                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, r.o[n][2 * b], 0, 0, 0);
-                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, r.o[n][2 * b + 1], 0, 0, 0);
-                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, r.o[n][2 * b], 0, 0, 0);
-                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, r.o[n][2 * b + 1], 0, 0, 0);
-                } else {
-                    const float back = __uint_as_float((uint32_t)(127 + down) << 23);
+                if constexpr (MODE == kApart) {
                     f4v t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, f4v{}, 0, 0, 0);
                     f4v z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, f4v{}, 0, 0, 0);
                     t = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, t, 0, 0, 0);
                     z = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, z, 0, 0, 0);
                     r.o[n][2 * b] += t * back;
                     r.o[n][2 * b + 1] += z * back;
+                } else {
+                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, r.o[n][2 * b], 0, 0, 0);
+                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, pl, r.o[n][2 * b + 1], 0, 0, 0);
+                    r.o[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, r.o[n][2 * b], 0, 0, 0);
+                    r.o[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, ph, r.o[n][2 * b + 1], 0, 0, 0);
                 }
             }
         }
@@ -753,22 +761,17 @@ __device__ __forceinline__ void kv4_few_keys(Kv4Few<NB>& r, const Kv4Raw<NB, 1>&
     const float corr = kv4_weights<MODE, 1>(s, r.factor, r.seen - key0 - 4 * L, r.m2, r.l);
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) r.o[i] *= corr;
-    int down = 0;   // powers of two that the column's products are formed below
-    if constexpr (MODE == kApart) down = kv4_down(x.vd[0]);
-    const float scale_down = __uint_as_float((uint32_t)(127 - down) << 23), back = __uint_as_float((uint32_t)(127 + down) << 23);
     h2v hi[4], lo[4];
+    float back = 1.f;   // of the column's products, formed apart
+    if constexpr (MODE == kApart) {
+        back = kv4_apart(s[0], x.vd[0], r.seen - key0 - 4 * L, hi, lo);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand
-        const int e = 4 * (i >> 1) + (i & 1);
-        const h2v d0 = as_h2(word_of(x.vd[0], e >> 1)), d1 = as_h2(word_of(x.vd[0], (e >> 1) + 1));
-        float f = (i & 1) ? d0.y : d0.x, h = (i & 1) ? d1.y : d1.x, p0 = s[0][e], p1 = s[0][e + 2];
-        if constexpr (MODE == kApart) {   // a key that the row does not see weighs 0 whatever its scale is
-            f = kv4::key_of(0, e) >= r.seen - key0 - 4 * L ? 0.f : f;
-            h = kv4::key_of(0, e + 2) >= r.seen - key0 - 4 * L ? 0.f : h;
-            p0 *= scale_down;
-            p1 *= scale_down;
+        for (int i = 0; i < 4; ++i) {   // slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand
+            const int e = 4 * (i >> 1) + (i & 1);
+            const h2v d0 = as_h2(word_of(x.vd[0], e >> 1)), d1 = as_h2(word_of(x.vd[0], (e >> 1) + 1));
+            split2(s[0][e], (i & 1) ? d0.y : d0.x, s[0][e + 2], (i & 1) ? d1.y : d1.x, hi[i], lo[i]);
         }
-        split2(p0, f, p1, h, hi[i], lo[i]);
     }
     const h8v ph = h8_of(hi[0], hi[1], hi[2], hi[3]), pl = h8_of(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
