@@ -395,20 +395,20 @@ __device__ __forceinline__ void kv4_rows_init(Kv4Rows<NB, NG>& r, const Kv4Attn&
 // that neither its scale nor what it holds matters.  A product that is no number
 // stays one (the maximum passes over it).
 __device__ __forceinline__ float kv4_apart(const float (&p)[8], const uint4& vs, int end, h2v (&hi)[4], h2v (&lo)[4]) {
-    float w[8], top = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    auto product = [&](int e) {   // formed twice: eight held between cost registers that the many-rows kernel has for q
         const h2v d = as_h2(word_of(vs, e >> 1));
-        w[e] = kv4::key_of(0, e) >= end ? 0.f : p[e] * (float)((e & 1) ? d.y : d.x);
-        top = fmaxf(top, fabsf(w[e]));
-    }
+        return kv4::key_of(0, e) >= end ? 0.f : p[e] * (float)((e & 1) ? d.y : d.x);
+    };
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(product(e)));
     top = over_groups_max(top);
     const int k = min(141 - (int)(__float_as_uint(top) >> 23), 126);
     const float up = __uint_as_float((uint32_t)(127 + k) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {   // slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand
         const int e = 4 * (i >> 1) + (i & 1);
-        split2(w[e], up, w[e + 2], up, hi[i], lo[i]);
+        split2(product(e), up, product(e + 2), up, hi[i], lo[i]);
     }
     return __uint_as_float((uint32_t)(127 - k) << 23);
 }
