@@ -78,6 +78,18 @@ def _run(ctx, K, Vv, n, q, G, scale, cap=None):
 
 
 @pytest.mark.parametrize("H,G,d,T", FEW + BLOCKS + TILES)
+@pytest.mark.parametrize("v_std", [1e-2, 1e-3, 1e-4, 1e-5, 1e-6])
+def test_small_values(ctx, v_std, H, G, d, T):
+    """Values of any size down to f16's smallest scales."""
+    print(f"[case] kv4 small values v={v_std} H={H} G={G} d={d} T={T}", flush=True)
+    n = max(T, 70)
+    K, Vv = F.normal(110, "k", n * G * d).reshape(n, -1), F.normal(110, "v", n * G * d, v_std).reshape(n, -1)
+    q = _queries(T, H, d, 110)
+    got = _run(ctx, K, Vv, n, q, G, 0.5)
+    _check(got, q, _stored(K, G, d)[0], *_stored(Vv, G, d), H, 0.5, 1, T > 100)
+
+
+@pytest.mark.parametrize("H,G,d,T", FEW + BLOCKS + TILES)
 @pytest.mark.parametrize("large", [30.0, 1e4, 1e5])
 def test_forgotten_large_values(ctx, large, H, G, d, T):
     """Finite large rows behind the context, left there by a truncation, beside small and usual values."""
@@ -122,6 +134,25 @@ def test_large_values_of_small_weight(ctx, weight, H, G, d, T):
     q[..., 0] = weight * (1 + 0.01 * F.normal(113, "q", T * H).reshape(T, H))
     got = _run(ctx, K.reshape(n, -1), Vv, n, q, G, 0.5)
     _check(got, q, _stored(K.reshape(n, -1), G, d)[0], *_stored(Vv, G, d), H, 0.5, 1, T > 100)
+
+
+@pytest.mark.parametrize("H,G,d,T", FEW + BLOCKS)
+def test_scales_at_the_borders(ctx, H, G, d, T):
+    """Scales on and next to 2^-11 and 2, zero, f16's smallest, its largest, and none that a row weighs alike."""
+    print(f"[case] kv4 borders H={H} G={G} d={d} T={T}", flush=True)
+    n = 97
+    K, Vv = F.normal(114, "k", n * G * d).reshape(n, -1), np.empty((n, G * d), np.float32)
+    step = 2.0 ** -10
+    scales = [2.0 ** -11, 2.0 ** -11 * (1 - step / 2), 2.0 ** -11 * (1 + step), 2.0, 2 * (1 - step / 2), 2 * (1 + step), 0.0, 2.0 ** -24,
+              3 * 2.0 ** -24, 2.0 ** -14, 65504.0, 1.0, 0.25]
+    codes = np.rint(F.normal(114, "c", n * G * d, 3.0)).clip(-7, 7).reshape(n, G * d // 32, 32)
+    codes[:, :, 5] = -8
+    for j in range(n):
+        for b in range(G * d // 32):
+            Vv[j, 32 * b:32 * b + 32] = codes[j, b] * scales[(j * 5 + b + j // 32) % len(scales)]
+    q = _queries(T, H, d, 114)
+    got = _run(ctx, K, Vv, n, q, G, 0.5)
+    _check(got, q, _stored(K, G, d)[0], *_stored(Vv, G, d), H, 0.5, 1, False)
 
 
 @pytest.mark.parametrize("H,G,d", [(32, 8, 128), (32, 4, 64)])

@@ -212,8 +212,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 //   weights  p = 2^(s - m + 10).  m moves when a score passes it by 4 (in powers of
 //            two), so p <= 2^14; rescaling O is rare and skipped by the wave.
 //   output   O^T = V^T P^T over the same codes: p times the key's scale, in two f16
-//            pieces, is the other operand.  It stays below 2^15 while scales are
-//            below 2.  Groups of 32 keys with a larger scale have their products formed
+//            pieces, is the other operand.  With scales from 2^-11 to below 2 (or 0) it
+//            stays below 2^15, and the second piece, which rounds at 2^-25 at the
+//            finest, is off by 2^-24 at most of the largest weight (2^10 or more) times the
+//            scale.  Groups of 32 keys with another scale have their products formed
 //            apart, each row's times the power of two that brings the largest that
 //            the row sees to [2^14, 2^15), and added scaled back: no key's scale costs
 //            another's bits, and a key that the row does not see has no say.
@@ -414,8 +416,8 @@ __device__ __forceinline__ float kv4_apart(const float (&p)[8], const uint4& vs,
 }
 
 // KG groups of 32 keys from key0 on; src: their operands (k, v) and scales (ks, vs) by
-// group and block.  kEdge: some row does not see all of them; kApart: as well, a value
-// block's scale is 2 or more (or no number).
+// group and block.  kEdge: some row does not see all of them; kApart: as well, values'
+// scales may be of any size (or no number).
 enum { kInside, kEdge, kApart };
 
 // A row's scores of KG groups of 32 keys, the lane's, become weights; m2 and l move on, and the
@@ -582,12 +584,13 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
 
 // A wave's share of 32 keys as it is loaded: lane (c, L) holds K words of keys c and
 // 16 + c, V bytes of elements 2c, 2c + 1 of each block for the keys of group L, and
-// those keys' scales, of NS blocks: all, or the one that the lane's column stands for.
+// those keys' scales, of NS blocks: all, or the one that the lane's column stands for; and one
+// word of V's scales of the group L for their size, which the lanes of L look at together.
 template <int NB, int NS = NB>
 struct Kv4Raw {
     uint32_t kw[2][NB], vw[2 * NB];
     uint4 kd[NS], vd[NS];
-    uint32_t magic;
+    uint32_t two, magic;
     static constexpr bool kValues = false;
 
     __device__ __forceinline__ void value(int, int, h8v&, h8v&) const {}
@@ -647,6 +650,7 @@ __device__ __forceinline__ void kv4_load(Kv4Raw<NB, NS>& r, const uint8_t* kc, c
 #pragma unroll
     for (int b = 0; b < NS; ++b)
         r.vd[b] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(tr, 16 * (L * NB + own + b), 0, 0));
+    r.two = __builtin_amdgcn_raw_buffer_load_b32(tr, 16 * L * NB + 4 * (c % (4 * NB)), 0, 0);
 }
 
 // A chunk's partial of a row: acc[D], m, l and two floats that align the next.  The host
@@ -842,33 +846,36 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
     constexpr std::integral_constant<int, kApart> apart;
     // Three loops of one body each (two in one would cost each other registers): the groups
     // that every row sees whole, those at some row's edge, and those of both that the first
-    // two left because of a large scale.
+    // two left because of a scale.
     bool left = false;
-    auto large = [&](const Raw& x) {   // a scale of 2 or more, or no number
-        uint32_t any = 0;
-#pragma unroll
-        for (int b = 0; b < (FEW ? 1 : NB); ++b) any |= x.vd[b].x | x.vd[b].y | x.vd[b].z | x.vd[b].w;
-        return __builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0;
+    // Of the lane's two scales one is 2 or more or no number (exponent bits 1xxxx), or below
+    // 2^-11 (000xx) and not 0.
+    auto is_apart = [&](const Raw& x) {
+        const uint32_t m = x.two & 0x7FFF7FFFu, not0 = (m + 0x7FFF7FFFu) >> 2;
+        return __builtin_amdgcn_ballot_w64(((m & 0x40004000u) | (not0 & ~(m | m << 1) & 0x20002000u)) != 0) != 0;
     };
     auto load = [&](int i) { kv4_load(raw, kc, vc, ks, vs, kb0 + i * stride, c, L, own); };   // i < mine
     int i = 0;
     for (; i < inside; ++i) {
         const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
-        if (large(cur)) left = true;
+        if (is_apart(cur)) left = true;
         else keys(whole, cur, i);
     }
     for (; i < mine; ++i) {
         const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
-        if (large(cur)) left = true;
+        if (is_apart(cur)) left = true;
         else keys(edge, cur, i);
     }
-    if (left)
+    if (left) {
+        load(0);
         for (i = 0; i < mine; ++i) {
-            load(i);
-            if (large(raw)) keys(apart, raw, i);
+            const Raw cur = raw;
+            if (i + 1 < mine) load(i + 1);
+            if (is_apart(cur)) keys(apart, cur, i);
         }
+    }
 
     // ---- the waves' results, then the chunk's ----
     float l, m;
