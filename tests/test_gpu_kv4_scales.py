@@ -6,7 +6,7 @@ Bounds (e = 2^-24, half an f32 step), all relative to what a row sees: scores,
 exponentials, sums and pieces as in the other tests of this cache, 2 e ((terms +
 16) S + n + 64) of sum p |v|.  Beside that a weight enters in two f16 pieces, whose
 second rounds at 2^-25 at the finest while the largest weight is 2^10 or more:
-  values in two pieces (many rows): 2^-35 |v| of each key, scales below 8192;
+  values in two pieces (many rows): 2^-35 |v| of each key, scales below 32;
   weights times scales (fewer rows), scales in [2^-11, 2): 2^-35 |code| <= e |v|;
   weights times scales, raised so that the largest of 32 keys is 2^14 or more: 2^-39 of
   that largest product times a code of up to 8, n 2^-36 max p D;
@@ -48,7 +48,7 @@ def _check(got, q, K, Vv, D, H, scale, terms, many):
         S = np.where(keep, np.abs(q[:, h]) @ np.abs(k).T * abs(float(scale)), 0).max(1, keepdims=True)
         floor = 2.0 ** -24 * keep @ (np.abs(v) * ((s >= 2.0 ** -11) & (s < 2)))
         if many:
-            floor += 2.0 ** -35 * keep @ (np.abs(v) * (s < 8192))
+            floor += 2.0 ** -35 * keep @ (np.abs(v) * (s < 32))
         floor += n * 2.0 ** -36 * np.stack([(p[t][:, None] * s).max(0) for t in range(T)])
         bound = (2 * 2.0 ** -24 * ((terms + 16) * S + n + 64) * (p @ np.abs(v)) + floor) / L
         ratio = np.abs(got[:, h] - p @ v / L) / bound
@@ -85,6 +85,18 @@ def test_small_values(ctx, v_std, H, G, d, T):
     n = max(T, 70)
     K, Vv = F.normal(110, "k", n * G * d).reshape(n, -1), F.normal(110, "v", n * G * d, v_std).reshape(n, -1)
     q = _queries(T, H, d, 110)
+    got = _run(ctx, K, Vv, n, q, G, 0.5)
+    _check(got, q, _stored(K, G, d)[0], *_stored(Vv, G, d), H, 0.5, 1, T > 100)
+
+
+@pytest.mark.parametrize("H,G,d,T", FEW + BLOCKS + TILES)
+@pytest.mark.parametrize("v_std", [5e-7, 2e-7])
+def test_smallest_values(ctx, v_std, H, G, d, T):
+    """Values whose scales are a few of f16's smallest steps, few keys."""
+    print(f"[case] kv4 smallest values v={v_std} H={H} G={G} d={d} T={T}", flush=True)
+    n = max(T, 40)
+    K, Vv = F.normal(116, "k", n * G * d).reshape(n, -1), F.normal(116, "v", n * G * d, v_std).reshape(n, -1)
+    q = _queries(T, H, d, 116)
     got = _run(ctx, K, Vv, n, q, G, 0.5)
     _check(got, q, _stored(K, G, d)[0], *_stored(Vv, G, d), H, 0.5, 1, T > 100)
 

@@ -554,7 +554,7 @@ __device__ __forceinline__ void kv4_keys(Kv4Rows<NB, NG>& r, const Src& src, int
                 float back = 1.f;
                 if constexpr (MODE == kApart) {
                     static_assert(KG == 1, "weights of one group of keys");
-                    back = kv4_apart(s[n][0], vs, r.seen[n] - key0 - 4 * L, hi, lo);
+                    back = kv4_apart(s[n][0], vs, r.seen[n] - key0 - 4 * L, hi, lo) * Src::kUp;
                 } else {
                     // Slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.
 #pragma unroll
@@ -592,6 +592,7 @@ struct Kv4Raw {
     uint4 kd[NS], vd[NS];
     uint32_t two, magic;
     static constexpr bool kValues = false;
+    static constexpr float kUp = 1.f;   // what O is held times
 
     __device__ __forceinline__ void value(int, int, h8v&, h8v&) const {}
     __device__ __forceinline__ h8v k(int, int u, int b) const {
@@ -995,16 +996,20 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
 // into LDS, where the operands stand as the lanes read them (a wave decodes a quarter of
 // the stage's K and of its V).  The next stage's codes are in registers meanwhile; the
 // other workgroup of the CU computes while this one decodes.  Values stand whole, as two
-// f16 pieces whose sum is exactly the code times the scale (15 bits) while the scale is
-// below 8192, so that only p is split, once for all blocks: three products for two, but
-// a quarter of the conversions, which cost more (16 cycles a weight and block).  Stages
-// with a larger scale, or one that is no number, come last, with codes and scales apart.
+// f16 pieces whose sum is exactly the code times the scale (15 bits) times 2^8, while the
+// scale is below 32, so that only p is split, once for all blocks: three products for two, but
+// a quarter of the conversions, which cost more (16 cycles a weight and block).  The 2^8,
+// which O carries and the last division takes back, lifts values of small scales out of
+// f16's subnormal range, whose products lose bits in the matrix cores' sums (values of
+// 1e-6: results 1e-5 off without it, as others with it).  Stages with a larger scale, or
+// one that is no number, come last, with codes and scales apart.
 // Each wave keeps its rows to the end, so nothing is merged.  Three passes, as above.
 // 1777 rows of 4001 keys at 32/8 heads of 128 226 us: 0.40 PFLOP/s of the attention's own
 // 91 GFLOP, 1.0 of the f16 products (two for a score, three for an output) where a
 // large product alone reaches 1.18.  A third product for the scores in place of the scaling
 // (K whole, in two pieces) took as long, one product for each took 28 % less.
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
+constexpr float kTileUp = 256.f;
 
 template <int NB>
 struct Kv4Stage {
@@ -1012,7 +1017,7 @@ struct Kv4Stage {
     uint4 k[16][64];               // [group][2][NB][lane]
     uint4 v[2][16][64];            // pieces of [group][NB][2][lane]; apart: codes in the first
     uint4 kd[32], vd[32];          // [group][L][block]; vd: apart only
-    uint32_t large[kTileWaves];    // a scale of 8192 or more among the wave's values
+    uint32_t large[kTileWaves];    // a scale of 32 or more among the wave's values
 };
 
 template <int NB>
@@ -1020,6 +1025,7 @@ struct Kv4FromStage {
     const Kv4Stage<NB>& st;
     int group, lane;
     static constexpr bool kValues = true;
+    static constexpr float kUp = kTileUp;
     __device__ __forceinline__ h8v k(int kg, int u, int b) const {
         return __builtin_bit_cast(h8v, st.k[(2 * (group + kg) + u) * NB + b][lane]);
     }
@@ -1101,8 +1107,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
                 if (c == 0) st.vd[(4 * vgroup + L) * NB + vblock + j] = vd[j];
             } else {
                 // The scales of slots (0, 2), (1, 3), (4, 6), (5, 7), as the codes stand.
-                const h2v d0 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x05040100)), d1 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x07060302));
-                const h2v d2 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x05040100)), d3 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x07060302));
+                const h2v up = {(_Float16)kTileUp, (_Float16)kTileUp};
+                const h2v d0 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x05040100)) * up, d1 = as_h2(__builtin_amdgcn_perm(vd[j].y, vd[j].x, 0x07060302)) * up;
+                const h2v d2 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x05040100)) * up, d3 = as_h2(__builtin_amdgcn_perm(vd[j].w, vd[j].z, 0x07060302)) * up;
                 auto both = [&](int to, h2v a0, h2v a1, h2v a2, h2v a3) {
                     const h2v h0 = a0 * d0, h1 = a1 * d1, h2 = a2 * d2, h3 = a3 * d3;
                     st.v[0][to][lane] = __builtin_bit_cast(uint4, h8_of(h0, h1, h2, h3));
@@ -1113,9 +1120,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
                 both(t + 1, x1, x3, y1, y3);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {   // exponent bits 111xx: 8192 and more
+            for (int i = 0; i < 4; ++i) {   // exponent bits 1x1xx or 11xxx: 32 and more
                 const uint32_t x = word_of(vd[j], i);
-                big |= x & (x << 1) & (x << 2);
+                big |= x & (x << 1 | x << 2);
             }
         }
         if (lane < 8) st.kd[8 * w + lane] = kd;
@@ -1179,7 +1186,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         const int row = row0 + 16 * n + c;
         if (row >= R) continue;
         const size_t at = kv4_row(a, g, row);
-        const float by = sum == 0.f ? 0.f : 1.f / sum;
+        const float by = sum == 0.f ? 0.f : 1.f / (sum * kTileUp);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
