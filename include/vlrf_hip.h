@@ -147,8 +147,11 @@ int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out
  * arguments, kernels and results; the chunks' partials go to one
  * fixed 2 MiB device array per GPU (resolved at vlrf_hip_init), so n_heads *
  * splits * (d_head + 2) floats must fit in 2^19 (splits = ceil(ctx_len / 64)),
- * otherwise VLRF_HIP_ERR_ARG; the per-head merge counters are the context's
- * (allocated at vlrf_hip_init).  Calls that overlap on one GPU race. */
+ * otherwise VLRF_HIP_ERR_ARG; a Q4_0 cache needs (d_head + 4) floats for each head and
+ * each workgroup that shares its keys, which fit for any context with up to 15 query heads
+ * a KV head or d_head 64 (with 16 / 1 heads of 128 up to 65536 tokens, 128 / 8 up to
+ * 8192).  The per-head merge counters are the context's (allocated at vlrf_hip_init).
+ * Calls that overlap on one GPU race. */
 int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, float* out,
                                  int n_heads, int ctx_len, float scale);
 /* Causal attention of T query rows, the last T of ctx_len tokens, over a Q4_0 cache

@@ -473,3 +473,56 @@ def test_refused_d_head_of_attention(ctx, d):
         assert rc == _lib.ERR_ARG and f"d_head {d}" in _lib.last_error()
     assert (out.download((3 * H * d,)) == 7).all()
     assert np.array_equal(kv.read(0, 0, n)[1].ravel(), F.quantize(x.download((n, d)), V.DT_Q4_0))
+
+
+@pytest.mark.parametrize("H,G,d,n", [(32, 8, 128, 8065), (32, 8, 128, 120001), (32, 4, 64, 30011), (15, 1, 128, 65600),
+                                     (16, 1, 64, 65600)])
+def test_decode_without_allocation_over_long_contexts(H, G, d, n):
+    """The call that allocates nothing at contexts where the other caches' partials would not fit, the
+    first call of its context and captured: the bits of the call with scratch."""
+    print(f"[case] kv4 noalloc H={H} G={G} d={d} n={n}", flush=True)
+    from test_gpu_prefill_gemm import _hip
+    hip, ctx, lib = _hip(), V.Context(0), V.lib()
+    assert H * ((n + 63) // 64) * (d + 2) > 1 << 19
+    row = G * d
+    x = ctx.to_device(F.normal(101, "rows", n * row))
+    kv = V.KVCache(ctx, 1, n, G, d, V.KV_Q4_0)
+    kv.append(0, x, x, n)
+    q, fix, out = ctx.to_device(F.normal(101, "q", H * d)), ctx.to_device(np.full(H * d + 5, 7, np.float32)), ctx.alloc(H * d * 4)
+    V.check(lib.vlrf_hip_attn_decode_noalloc(kv.h, 0, q.ptr, fix.ptr, H, n, C.c_float(0.1)))
+    got = fix.download((H * d + 5,))
+    kv.attention_decode(0, q, out, H, n, 0.1)
+    assert np.array_equal(got[:H * d], out.download((H * d,))) and (got[H * d:] == 7).all() and np.abs(got[:H * d]).max() > 0
+    s, g, ge = C.c_void_p(ctx.stream()), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(s, 2) == 0
+    try:
+        rc = lib.vlrf_hip_attn_decode_noalloc(kv.h, 0, q.ptr, fix.ptr, H, n, C.c_float(0.1))
+    finally:
+        end = hip.hipStreamEndCapture(s, C.byref(g))
+    assert rc == 0 and end == 0
+    assert hip.hipGraphInstantiate(C.byref(ge), g, None, None, 0) == 0
+    for i in range(3):
+        fix.zero()
+        kv.attention_decode(0, q, out, H, n - 1 - i, 0.1)
+        assert hip.hipGraphLaunch(ge, s) == 0
+        ctx.sync()
+        assert np.array_equal(fix.download((H * d,)), got[:H * d])
+    hip.hipGraphExecDestroy(ge)
+    hip.hipGraphDestroy(g)
+
+
+def test_decode_without_allocation_refuses_what_does_not_fit(ctx):
+    """16 query heads of 128 on one KV head: 256 workgroups' partials are more than the fixed array."""
+    H, n = 16, 65600
+    x = ctx.to_device(F.normal(102, "rows", n * 128))
+    kv = V.KVCache(ctx, 1, n, 1, 128, V.KV_Q4_0)
+    kv.append(0, x, x, n)
+    q, out = ctx.to_device(F.normal(102, "q", H * 128)), ctx.to_device(np.full(H * 128, 7, np.float32))
+    for m in (65537, n):
+        rc = V.lib().vlrf_hip_attn_decode_noalloc(kv.h, 0, q.ptr, out.ptr, H, m, C.c_float(0.1))
+        assert rc == _lib.ERR_ARG and "exceed the fixed scratch" in _lib.last_error()
+        assert (out.download((H * 128,)) == 7).all()
+    assert V.lib().vlrf_hip_attn_decode_noalloc(kv.h, 0, q.ptr, out.ptr, H, 65536, C.c_float(0.1)) == 0
+    got = out.download((H * 128,))
+    kv.attention_decode(0, q, out, H, 65536, 0.1)
+    assert np.array_equal(out.download((H * 128,)), got)

@@ -83,3 +83,20 @@ def test_scratch_of_refused_attention_is_none():
             "print('ok')" % ROOT)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "ok", (r.returncode, r.stderr[-800:])
+
+
+def test_fixed_scratch_serves_long_contexts():
+    """What a decode row's partials need beside the 2^19 floats of the call that allocates nothing: less at
+    any context with up to 15 query heads a KV head or heads of 64."""
+    part = V.lib()._ZN8vlrf_hip19attn_kv4_part_bytesEiiiii
+    part.restype, part.argtypes = C.c_size_t, [C.c_int] * 5
+    for d in (64, 128):
+        for G in (1, 2, 3, 4, 8, 16, 40):
+            for rep in range(1, 41):
+                for n in (1, 256, 257, 8065, 20000, 65536, 65537, 120001, 1 << 20, 1 << 27):
+                    need = part(G * rep, G, d, 1, n) // 4
+                    assert need <= 256 * 16 * (d + 4)
+                    if d == 64 or rep < 16:
+                        assert need <= 1 << 19, (G, rep, d, n)
+    for H, G, n in ((16, 1, 65536), (128, 8, 8192)):
+        assert part(H, G, 128, 1, n) // 4 <= 1 << 19 < part(H, G, 128, 1, n + 1) // 4

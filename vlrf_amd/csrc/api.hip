@@ -665,15 +665,20 @@ int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, fl
            kv->max_seq);
     VH_ARG(n_heads >= 1, "attn_decode_noalloc: n_heads %d", n_heads);
     VH_ARG(kv->ctx->noalloc_scratch != nullptr, "attn_decode_noalloc: context has no fixed scratch");
+    const KVLayer& L = kv->layers[layer];
+    if (L.dtype == VLRF_HIP_KV_Q4_0) {
+        const size_t need = attn_kv4_part_bytes(n_heads, kv->n_kv, kv->d_head, 1, ctx_len) / sizeof(float);
+        VH_ARG(need <= noalloc::kScratchFloats,
+               "attn_decode_noalloc: %zu partial floats (n_heads %d of %d keys, n_kv %d) exceed the fixed scratch of %zu", need,
+               n_heads, ctx_len, kv->n_kv, noalloc::kScratchFloats);
+        return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out,
+                               kv->ctx->noalloc_scratch, kv->ctx->small_tile_ctr);
+    }
     const int splits = attn_decode_splits(ctx_len);
     const size_t need = (size_t)n_heads * splits * (kv->d_head + 2);
     VH_ARG(need <= noalloc::kScratchFloats,
            "attn_decode_noalloc: %zu partial floats (n_heads %d x %d splits x %d) exceed the fixed scratch of %zu",
            need, n_heads, splits, kv->d_head + 2, noalloc::kScratchFloats);
-    const KVLayer& L = kv->layers[layer];
-    if (L.dtype == VLRF_HIP_KV_Q4_0)
-        return launch_attn_kv4(kv->ctx->stream, q, L, n_heads, kv->n_kv, kv->d_head, kv->max_seq, 1, ctx_len, scale, out,
-                               kv->ctx->noalloc_scratch, kv->ctx->small_tile_ctr);
     return launch_attn_decode(kv->ctx->stream, q, L.k, L.v, L.ks, L.vs, L.dtype, (long)kv->max_seq * kv->d_head,
                               n_heads, kv->n_kv, kv->d_head, ctx_len, nullptr, splits, scale,
                               kv->ctx->noalloc_scratch, out, nullptr, kv->ctx->small_tile_ctr);
