@@ -118,21 +118,33 @@ class _Buffer:
 _CONTEXT = []
 
 
-def _handle(case, old):
-    """The framework's cache with the rows that are in it before the call."""
+def _context():
     import vlrf_amd as V
     if not _CONTEXT:                   # one context for the program, as a server keeps it
         _CONTEXT.append(V.Context(0))
+    return _CONTEXT[0]
+
+
+def _handle(case, old):
+    """The framework's cache with the rows that are in it before the call."""
+    import vlrf_amd as V
     n = case["base"] + case["T"] if case["op"] == "write" else case["ctx"]
-    cache = V.KVCache(_CONTEXT[0], 1, n, case["G"], case["d"], dtype=V.KV_Q4_0)
+    cache = V.KVCache(_context(), 1, n, case["G"], case["d"], dtype=V.KV_Q4_0)
     if old is not None:
-        torch.cuda.synchronize()
         cache.append(0, _Buffer(old[0]), _Buffer(old[1]), old[0].shape[0])
-        torch.cuda.synchronize()
     return cache
 
 
 def prepare(case, seed):
+    if not own:
+        return _prepare(case, seed)
+    # The context's stream is not ordered with torch's: inputs are made on it, and outputs belong to
+    # it, so that the calls come after the inputs and no tensor is used again before they are done.
+    with torch.cuda.stream(torch.cuda.ExternalStream(_context().stream())):
+        return _prepare(case, seed)
+
+
+def _prepare(case, seed):
     old, new, q = _inputs(case, seed)
     n = case["base"] + case["T"] if case["op"] == "write" else case["ctx"]
     width = case["G"] * case["d"]
@@ -218,6 +230,8 @@ def _calls(state):
 
 
 def run(state):
+    """One pass.  The framework's calls are queued on its context's stream: what they return is
+    there after Context.sync() or torch.cuda.synchronize()."""
     return _calls(state) if own else _plain(state)
 
 
