@@ -526,3 +526,51 @@ def test_decode_without_allocation_refuses_what_does_not_fit(ctx):
     got = out.download((H * 128,))
     kv.attention_decode(0, q, out, H, 65536, 0.1)
     assert np.array_equal(out.download((H * 128,)), got)
+
+
+def test_scratch_does_not_grow_under_capture():
+    """Calls whose partials need more scratch than the context holds are an error while its stream is
+    captured, and the capture goes on; after the same call once before, they are recorded."""
+    from test_gpu_prefill_gemm import _hip
+    hip, ctx, lib = _hip(), V.Context(0), V.lib()
+    H, G, d, n = 32, 8, 128, 3000
+    x = ctx.to_device(F.normal(103, "rows", n * G * d))
+    kv = V.KVCache(ctx, 1, n, G, d, V.KV_Q4_0)
+    kv.append(0, x, x, n)
+    q, outs = ctx.to_device(F.normal(103, "q", 5 * H * d)), [ctx.to_device(np.full(5 * H * d, 7, np.float32)) for _ in range(2)]
+    s = C.c_void_p(ctx.stream())
+
+    def calls():
+        return [lib.vlrf_hip_attn_decode(kv.h, 0, q.ptr, outs[0].ptr, H, n, C.c_float(0.1)),
+                lib.vlrf_hip_attn_chunk(kv.h, 0, q.ptr, outs[1].ptr, H, 5, n, C.c_float(0.1))]
+
+    def captured():
+        g = C.c_void_p()
+        assert hip.hipStreamBeginCapture(s, 2) == 0
+        try:
+            rcs, said = calls(), _lib.last_error()
+        finally:
+            rc = hip.hipStreamEndCapture(s, C.byref(g))
+        assert rc == 0
+        return rcs, said, g
+
+    rcs, said, g = captured()
+    assert rcs == [_lib.ERR_ARG] * 2 and "captured" in said
+    hip.hipGraphDestroy(g)
+    assert all((o.download((5 * H * d,)) == 7).all() for o in outs)
+    assert calls() == [0, 0]
+    want = [o.download((5 * H * d,)) for o in outs]
+    rcs, _, g = captured()
+    assert rcs == [0, 0]
+    ge = C.c_void_p()
+    assert hip.hipGraphInstantiate(C.byref(ge), g, None, None, 0) == 0
+    for i in range(3):
+        for o in outs:
+            o.zero()
+        kv.attention_decode(0, q, outs[0], H, n - 1 - i, 0.1)
+        assert hip.hipGraphLaunch(ge, s) == 0
+        ctx.sync()
+        got = [o.download((5 * H * d,)) for o in outs]
+        assert np.array_equal(got[0][:H * d], want[0][:H * d]) and np.array_equal(got[1], want[1])
+    hip.hipGraphExecDestroy(ge)
+    hip.hipGraphDestroy(g)
