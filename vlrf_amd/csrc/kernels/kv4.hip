@@ -847,8 +847,8 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
     constexpr std::integral_constant<int, kApart> apart;
     // Three loops of one body each (two in one would cost each other registers): the groups
     // that every row sees whole, those at some row's edge, and those of both that the first
-    // two left because of a scale.
-    bool left = false;
+    // two left because of a scale, which the third looks for between the first and the last of them.
+    int from = mine, to = 0;
     // Of the lane's two scales one is 2 or more or no number (exponent bits 1xxxx), or below
     // 2^-11 (000xx) and not 0.
     auto is_apart = [&](const Raw& x) {
@@ -860,22 +860,20 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
     for (; i < inside; ++i) {
         const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
-        if (is_apart(cur)) left = true;
+        if (is_apart(cur)) from = min(from, i), to = i + 1;
         else keys(whole, cur, i);
     }
     for (; i < mine; ++i) {
         const Raw cur = raw;
         if (i + 1 < mine) load(i + 1);
-        if (is_apart(cur)) left = true;
+        if (is_apart(cur)) from = min(from, i), to = i + 1;
         else keys(edge, cur, i);
     }
-    if (left) {
-        load(0);
-        for (i = 0; i < mine; ++i) {
-            const Raw cur = raw;
-            if (i + 1 < mine) load(i + 1);
-            if (is_apart(cur)) keys(apart, cur, i);
-        }
+    if (from < to) load(from);
+    for (i = from; i < to; ++i) {
+        const Raw cur = raw;
+        if (i + 1 < to) load(i + 1);
+        if (is_apart(cur)) keys(apart, cur, i);
     }
 
     // ---- the waves' results, then the chunk's ----
@@ -1150,10 +1148,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
         kv4_query<NB>(q, a, g, min(row0 + 16 * n + c, R - 1), L);   // rows past the last one repeat it and are not stored
         kv4_rows_init<NB, NG>(r, a, q, n);
     }
-    bool left = false;
+    int from = end, to = 0;   // the stages left for the last pass lie between
     stages(std::false_type(), 0, inside, [&](int s) {
         if (is_large()) {
-            left = true;
+            from = min(from, s), to = s + 1;
             return;
         }
 #pragma unroll
@@ -1162,7 +1160,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
     });
     stages(std::false_type(), inside, end, [&](int s) {
         if (is_large()) {
-            left = true;
+            from = min(from, s), to = s + 1;
             return;
         }
 #pragma unroll 1
@@ -1171,15 +1169,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void kv4_attn_tiles_kernel(Kv4A
             if (key0 < most) kv4_keys<kEdge, 2>(r, Kv4FromStage<NB>{st, 2 * i, lane}, key0, L);
         }
     });
-    if (left)
-        stages(std::true_type(), 0, end, [&](int s) {
-            if (!is_large()) return;
+    stages(std::true_type(), from, to, [&](int s) {
+        if (!is_large()) return;
 #pragma unroll 1
-            for (int i = 0; i < Stage::GROUPS; ++i) {
-                const int key0 = s * Stage::KEYS + 32 * i;
-                if (key0 < most) kv4_keys<kApart, 1>(r, Kv4FromStage<NB>{st, i, lane}, key0, L);
-            }
-        });
+        for (int i = 0; i < Stage::GROUPS; ++i) {
+            const int key0 = s * Stage::KEYS + 32 * i;
+            if (key0 < most) kv4_keys<kApart, 1>(r, Kv4FromStage<NB>{st, i, lane}, key0, L);
+        }
+    });
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
         const float sum = over_groups_sum(r.l[n]);
