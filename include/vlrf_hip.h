@@ -135,8 +135,9 @@ int vlrf_hip_kv_dequant(vlrf_hip_kv_t kv, int layer, int ctx_len, float* K_out, 
  * d_head 64, ctx_len <= 8192 and less than 8 MiB of K/V one launch (each head's
  * context in at most 16 chunks, merged by the head's last workgroup), else one
  * that reads K/V once per four query heads and, over more than one chunk, a merge.
- * A Q4_0 cache at any length: one launch, K/V read once (vlrf_hip_attn_chunk's), and
- * a merge where more than 32 workgroups share the keys of a KV head.
+ * A Q4_0 cache at any length: one launch, K/V read once per 16 query heads of a KV
+ * head (4, at d_head 64 8, where there are no more or the context is short), and a merge
+ * where more than 32 workgroups share the keys; accuracy as vlrf_hip_attn_chunk's.
  * Replaces the decode branch of AttentionBlock::forward: dequant_into +
  * reshape/expand_kv_heads + sdp_heads (attention.hpp:127-176). */
 int vlrf_hip_attn_decode(vlrf_hip_kv_t kv, int layer, const float* q, float* out,
@@ -158,9 +159,14 @@ int vlrf_hip_attn_decode_noalloc(vlrf_hip_kv_t kv, int layer, const float* q, fl
  * (a prompt in chunks, or drafted tokens checked together; their K/V are appended
  * first): q and out device f32 [T, n_heads*d_head], q already rotated; row t sees the
  * keys [0, ctx_len - T + t].  1 <= T <= ctx_len <= max_seq; d_head 64 or 128; any
- * n_heads / n_kv_heads.  Other cache dtypes are VLRF_HIP_ERR_ARG.  f32-class: q and
- * the weights enter the matrix cores in two f16 pieces (22 bits) beside the cache's
- * exact codes, sums and softmax in f32.  attn_decode over a Q4_0 cache is T = 1. */
+ * n_heads / n_kv_heads.  Other cache dtypes are VLRF_HIP_ERR_ARG, and so are q and out
+ * that overlap.  f32-class: q and the weights enter the matrix cores in two f16 pieces
+ * (22 bits; an element of q no finer than 2^-38 of its row's largest, a weight times its
+ * value no finer than 2^-24 of the row's largest weight times that value or 2^-36 of the
+ * largest such product within its 32 keys) beside the cache's exact codes, sums and softmax
+ * in f32.  Keys that a row does not see have no effect whatever they hold.  A call over
+ * blocks whose largest value is under 2^-8, or 16 or more, takes up to twice as long.
+ * attn_decode over a Q4_0 cache is T = 1. */
 int vlrf_hip_attn_chunk(vlrf_hip_kv_t kv, int layer, const float* q, float* out, int n_heads, int T,
                         int ctx_len, float scale);
 

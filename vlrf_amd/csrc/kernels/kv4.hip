@@ -201,8 +201,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 // four waves of each take groups of 32 keys in turn, each with its own running maximum
 // and sum, and merge through LDS, and the workgroup that comes last merges all of a
 // block's.
-// One decode row at 32/8 heads of 128: 120001 keys 34.5 us (138 MB, 4.0 TB/s, what a large
-// read reaches); 15001 keys 10.0 (17 MB, 1.7 TB/s) and 1500 keys 6.8, bound by the chain of
+// One decode row at 32/8 heads of 128: 120001 keys 33.9 us (138 MB, 4.1 TB/s: each byte read
+// once, a wave with one group of keys in flight waits 39 % of its time and vector
+// instructions take half of every SIMD's; a GEMV of this library reads at 5.1 TB/s); 15001
+// keys 9.7 (17 MB, 1.8 TB/s) and 1500 keys 6.7, bound by the chain of
 // waits: the launch, the arguments, q and the keys, the group's products and weights, the waves'
 // merge, the counter, the chunks' merge, 0.3 to 0.9 us each.
 //   scores   S^T = K Q^T, 16 keys by 16 rows and a block of 32 elements an
@@ -218,7 +220,10 @@ __global__ __launch_bounds__(256) void kv4_dequant_kernel(const uint8_t* __restr
 //            scale.  Groups of 32 keys with another scale have their products formed
 //            apart, each row's times the power of two that brings the largest that
 //            the row sees to [2^14, 2^15), and added scaled back: no key's scale costs
-//            another's bits, and a key that the row does not see has no say.
+//            another's bits, and a key that the row does not see has no say.  Where
+//            every group goes that way (values of 1e-3, or of 1e4) a call takes up
+//            to twice as long: 120001 keys 31 -> 55 us, 15001 9.8 -> 10.9, 200 rows of
+//            4200 64 -> 118; where only the first key's scale is such a one, under 1 us.
 // A lane's scores are of the row that is its column in both products and of the keys
 // that its group of V's layout holds, so nothing moves between lanes but the
 // maximum's two exchanges a group.
@@ -1002,10 +1007,14 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
 // 1e-6: results 1e-5 off without it, as others with it).  Stages with a larger scale, or
 // one that is no number, come last, with codes and scales apart.
 // Each wave keeps its rows to the end, so nothing is merged.  Three passes, as above.
-// 1777 rows of 4001 keys at 32/8 heads of 128 226 us: 0.40 PFLOP/s of the attention's own
+// 1777 rows of 4001 keys at 32/8 heads of 128 225 us: 0.40 PFLOP/s of the attention's own
 // 91 GFLOP, 1.0 of the f16 products (two for a score, three for an output) where a
-// large product alone reaches 1.18.  A third product for the scores in place of the scaling
-// (K whole, in two pieces) took as long, one product for each took 28 % less.
+// large product alone reaches 1.17.  Counted over all SIMDs and the whole launch, matrix
+// instructions take 36 % and other vector ones 35 %, the CUs hold work 76 % of the time:
+// the two hardly overlap.  At d_head 64 (2500 rows of 2500 at 32/4 heads 97 us) 24 and 34 %
+// of 64 %: half the products a key, but the same softmax and split of p.  A third product for
+// the scores in place of the scaling (K whole, in two pieces) took as long, one product for
+// each took 28 % less.
 constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 constexpr float kTileUp = 256.f;
 
